@@ -236,6 +236,91 @@ pa_status pa_qk_norm_rope_and_cache(PagedAttnCache *cache, uint32_t layer_idx,
                                     int64_t k_stride, int64_t v_stride,
                                     void *cuda_stream);
 
+/* Rotation plan: which elements of a head turn, in which pairs, how fast.  A host object
+ * without device state, read-only once made: any number of caches, streams and threads
+ * may use one plan.  No counterpart in the reference, whose rotation is fast::rope with
+ * fixed arguments (crates/mlx-sys/src/mlx.cpp:1343-1365).
+ *   rope_dims    elements of a head that turn (the first ones), even, 2..256
+ *   interleaved  0: element i pairs with i + rope_dims/2; 1: element 2i with 2i + 1
+ *   base         pair i turns by f_i = base^(-i / (rope_dims/2)) radians per position
+ *   scaling      what a longer context than the trained one does to f_i:
+ *     PLAIN   nothing
+ *     LINEAR  f_i / factor
+ *     BANDS   with n_i = original_max_position * f_i / (2 pi) turns over the trained
+ *             length and k = clamp((n_i - low_freq_factor) / (high_freq_factor -
+ *             low_freq_factor), 0, 1): k f_i + (1 - k) f_i / factor
+ *     YARN    a ramp over i between the indexes whose pairs make beta_fast and beta_slow
+ *             turns over the trained length (rounded down and up): f_i before it,
+ *             f_i / factor behind it, a blend on it
+ *   attention_factor  multiplies sine and cosine; 0 stands for 1, with YARN and a factor
+ *             above 1 for 0.1 ln(factor) + 1
+ * Fields that the scaling does not name are not looked at.                         */
+enum { PA_ROPE_PLAIN = 0, PA_ROPE_LINEAR = 1, PA_ROPE_BANDS = 2, PA_ROPE_YARN = 3 };
+typedef struct PaRopeConfig {
+  uint32_t rope_dims;
+  uint32_t interleaved;
+  float base;
+  uint32_t scaling;
+  float factor;
+  uint32_t original_max_position;
+  float low_freq_factor, high_freq_factor; /* BANDS */
+  float beta_fast, beta_slow;              /* YARN */
+  float attention_factor;
+} PaRopeConfig;
+typedef struct PaRope PaRope; /* opaque */
+pa_status pa_rope_create(const PaRopeConfig *config, PaRope **out_rope);
+pa_status pa_rope_free(PaRope *rope);
+/* Radians per position of every pair (rope_dims/2 doubles) and the gain; either may be null. */
+pa_status pa_rope_frequencies(const PaRope *rope, double *frequencies, float *gain);
+
+/* Per-head RMS norm of queries and keys, rotation and cache write by a plan, one launch
+ * for all tokens.  Next to pa_qk_norm_rope_and_cache it takes every head size, block size
+ * and cache type of the library, both pair layouts and scaled frequencies, can leave the
+ * keys in a buffer too, and differs in two points of its arithmetic: a row is computed in
+ * fp32 from end to end and rounded once, to the 16-bit type (the other call rounds after
+ * the norm and after the weight, as the reference does), and a position's angle is reduced
+ * in 64-bit fixed point, so that it is as exact at position 2^31 as at 1.
+ *   rope         plan with rope_dims <= head_size
+ *   q, k, v      [num_tokens, heads, head_size] in the cache dtype, row strides in
+ *                elements (the parts of one fused projection output, for instance)
+ *   q_out        receives the queries; may be q itself with q's stride
+ *   k_out        null, or receives the keys [num_tokens, num_kv_heads, head_size]; may be k
+ *                itself with k's stride.  No other overlap of inputs and outputs is allowed
+ *   q_norm_weight, k_norm_weight  [head_size] in the cache dtype, or null for no norm
+ *   positions    int32 [num_tokens], device; any value
+ *   slot_mapping int64 [num_tokens], device, or null: nothing is written to the pool (v may
+ *                then be null).  Skipping and reporting as in pa_reshape_and_cache; of two
+ *                tokens with one slot either may be the one that stays
+ * The pool bytes after the call are those pa_reshape_and_cache would have written from
+ * k_out and v (an FP8 cache quantises the 16-bit key with the layer's scales).     */
+pa_status pa_rope_norm_and_cache(PagedAttnCache *cache, uint32_t layer_idx, const PaRope *rope,
+                                 void *q_out, void *k_out, const void *q, const void *k,
+                                 const void *v, const void *q_norm_weight,
+                                 const void *k_norm_weight, float eps, const int32_t *positions,
+                                 const int64_t *slot_mapping, int64_t num_tokens,
+                                 int32_t num_q_heads, int64_t q_stride, int64_t q_out_stride,
+                                 int64_t k_stride, int64_t k_out_stride, int64_t v_stride,
+                                 void *cuda_stream);
+
+/* Read-back: the cached keys and values of token ranges as packed 16-bit rows, the inverse
+ * of the cache write (an FP8 cache is decoded and multiplied by the layer's scales).  For a
+ * prompt whose prefix is cached (pa_prompt_attention below), for moving a sequence to
+ * another cache, for looking at what a cache holds.
+ *   key, value    [.., num_kv_heads, head_size] in the cache dtype, row strides in elements:
+ *                 row cu_lens[s] + i receives token starts[s] + i of sequence s
+ *   block_tables  int32 [num_seqs, max_blocks_per_seq], device
+ *   starts_host   int32 [num_seqs] in HOST memory: first token of each range, or null (0)
+ *   cu_lens_host  int32 [num_seqs + 1] in HOST memory, non-decreasing; the rows from
+ *                 cu_lens[0] on are written, no others
+ * The two host arrays are read during the call only.  A block id outside the pool is not
+ * followed: its rows are left as they were and pa_cache_check_errors reports
+ * PA_ERR_OUT_OF_RANGE.                                                             */
+pa_status pa_gather_cache(PagedAttnCache *cache, uint32_t layer_idx, void *key, void *value,
+                          const int32_t *block_tables, const int32_t *starts_host,
+                          const int32_t *cu_lens_host, int32_t num_seqs,
+                          int32_t max_blocks_per_seq, int64_t key_stride, int64_t value_stride,
+                          void *cuda_stream);
+
 /* Copy-on-write block copy.  dispatch_copy_blocks_raw
  * (crates/mlx-paged-attn/src/metal/copy_blocks.rs:96-99) over
  * crates/mlx-paged-attn/metal/cache/copy_blocks.metal:6-36.
@@ -458,6 +543,36 @@ pa_status pa_paged_attention_varlen(PagedAttnCache *cache, uint32_t layer_idx,
                                     float softcap, int32_t max_context_len,
                                     void *workspace, size_t workspace_bytes,
                                     void *cuda_stream);
+
+/* Causal attention of packed prompts over CONTIGUOUS keys and values - a prompt straight
+ * from its projections, or a chunk over a prefix that pa_gather_cache or
+ * pa_rope_norm_and_cache left in a buffer - with the semantics of
+ * pa_paged_attention_varlen: sequence s has kv_len = cu_kv_lens[s+1] - cu_kv_lens[s] keys
+ * and q_len queries on its last positions; query j sees keys [0, kv_len - q_len + j].  A
+ * query that sees none (kv_len < q_len) gives a zero row.  The reference runs its dense
+ * prefill one sequence at a time (crates/mlx-core/src/transformer/block.rs:279-317).
+ * Every head size of the library; head size, kv heads and dtype are the cache's (an FP8
+ * cache's q/out type), its pools are not touched.
+ *   out, q        [cu_q_lens[num_seqs], num_q_heads, head_size], packed by sequence
+ *   k, v          [cu_kv_lens[num_seqs], num_kv_heads, head_size]; row strides of all four
+ *                 in elements
+ *   cu_q_lens_host, cu_kv_lens_host  int32 [num_seqs + 1] in HOST memory, non-decreasing,
+ *                 read during the call only (a captured graph replays these lengths);
+ *                 cu_kv_lens_host may be null: the same as cu_q_lens_host
+ *   num_q_heads   a multiple of num_kv_heads, at most 128 times it
+ *   softcap       1.0f = off
+ *   workspace     >= pa_prompt_workspace_bytes(), 256-byte aligned, device; not shared by
+ *                 calls that may run at the same time
+ * What a masked key or value holds, NaN and infinity among it, does not reach a row that
+ * does not see it.  Results do not depend on anything but the arguments and the GPU's SM
+ * count: the same call gives the same bits.                                         */
+size_t pa_prompt_workspace_bytes(const PagedAttnCache *cache);
+pa_status pa_prompt_attention(PagedAttnCache *cache, void *out, const void *q, const void *k,
+                              const void *v, const int32_t *cu_q_lens_host,
+                              const int32_t *cu_kv_lens_host, int32_t num_seqs,
+                              int32_t num_q_heads, int64_t q_stride, int64_t k_stride,
+                              int64_t v_stride, int64_t out_stride, float scale, float softcap,
+                              void *workspace, size_t workspace_bytes, void *cuda_stream);
 
 /* One decode step of one layer from HOST buffers, the order
  * TransformerBlock::forward_paged keeps (crates/mlx-core/src/transformer/

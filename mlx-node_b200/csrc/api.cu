@@ -15,6 +15,7 @@
 
 #include "../../include/paged_attn_b200.h"
 #include "pa_common.cuh"
+#include "prompt_path.cuh"
 
 namespace {
 
@@ -179,6 +180,7 @@ pa_status finish_create(PagedAttnCache *c) {
   PA_CUDA(pa::splitkv_configure());
   PA_CUDA(pa::tile_configure());
   PA_CUDA(pa::tile64_configure());
+  PA_CUDA(pa::prompt_configure());
   // the tile kernel fetches V of 16-bit pools through a tensor map (FP8 pools are read with
   // plain loads: their entries stay zero and unused)
   c->v_maps.assign(c->cfg.num_layers, pa::TensorMapBlob{});
@@ -543,6 +545,187 @@ pa_status pa_qk_norm_rope_and_cache(PagedAttnCache *c, uint32_t layer, void *q_o
   DeviceGuard g(c->device);
   PA_CUDA(pa::launch_qk_norm_rope_cache(p, c->cfg.dtype == 0, c->num_sms,
                                         static_cast<cudaStream_t>(cuda_stream)));
+  return PA_OK;
+}
+
+/* ---- prompt path: rotation + cache write, read-back, packed prompt attention -------- */
+}  // extern "C"
+
+struct PaRope {
+  PaRopeConfig cfg{};
+  pa::RopeTable table{};
+};
+
+namespace {
+pa_status arg_fail(const pa::ArgError &e) { return fail(e.code, e.what); }
+}  // namespace
+
+extern "C" {
+
+pa_status pa_rope_create(const PaRopeConfig *config, PaRope **out_rope) {
+  if (!out_rope) return fail(PA_ERR_INVALID_ARG, "out_rope is null");
+  *out_rope = nullptr;
+  if (!config) return fail(PA_ERR_INVALID_ARG, "config is null");
+  if (pa::ArgError e = pa::check_rope_config(*config)) return arg_fail(e);
+  PaRope *r = new (std::nothrow) PaRope();
+  if (!r) return fail(PA_ERR_OOM, "host allocation failed");
+  r->cfg = *config;
+  pa::build_rope_table(*config, &r->table);
+  *out_rope = r;
+  return PA_OK;
+}
+pa_status pa_rope_free(PaRope *rope) {
+  delete rope;
+  return PA_OK;
+}
+pa_status pa_rope_frequencies(const PaRope *rope, double *frequencies, float *gain) {
+  if (!rope) return fail(PA_ERR_INVALID_ARG, "rope plan is null");
+  if (frequencies)
+    for (int i = 0; i < (int)rope->cfg.rope_dims / 2; i++)
+      frequencies[i] = (double)pa::rope_frequency(rope->cfg, i);
+  if (gain) *gain = rope->table.gain;
+  return PA_OK;
+}
+
+pa_status pa_rope_norm_and_cache(PagedAttnCache *c, uint32_t layer, const PaRope *rope, void *q_out,
+                                 void *k_out, const void *q, const void *k, const void *v,
+                                 const void *q_norm_weight, const void *k_norm_weight, float eps,
+                                 const int32_t *positions, const int64_t *slot_mapping,
+                                 int64_t num_tokens, int32_t num_q_heads, int64_t q_stride,
+                                 int64_t q_out_stride, int64_t k_stride, int64_t k_out_stride,
+                                 int64_t v_stride, void *cuda_stream) {
+  pa_status st = check_layer(c, layer);
+  if (st != PA_OK) return st;
+  if (num_tokens < 0) return fail(PA_ERR_INVALID_ARG, "num_tokens < 0");
+  if (num_tokens == 0) return PA_OK;
+  if (pa::ArgError e = pa::check_rotate_args(c->cfg, rope ? &rope->table : nullptr, q_out, k_out, q, k, v,
+                                             q_norm_weight, k_norm_weight, eps, positions, slot_mapping,
+                                             num_tokens, num_q_heads, q_stride, q_out_stride, k_stride,
+                                             k_out_stride, v_stride))
+    return arg_fail(e);
+  pa::RotateParams p{};
+  p.q = static_cast<const pa::elem16 *>(q);
+  p.k = static_cast<const pa::elem16 *>(k);
+  p.v = static_cast<const pa::elem16 *>(v);
+  p.q_out = static_cast<pa::elem16 *>(q_out);
+  p.k_out = static_cast<pa::elem16 *>(k_out);
+  p.q_norm_w = static_cast<const pa::elem16 *>(q_norm_weight);
+  p.k_norm_w = static_cast<const pa::elem16 *>(k_norm_weight);
+  p.positions = positions;
+  p.slot_mapping = slot_mapping;
+  p.k_pool = c->k[layer];
+  p.v_pool = c->v[layer];
+  p.num_tokens = num_tokens;
+  p.q_stride = q_stride;
+  p.q_out_stride = q_out_stride;
+  p.k_stride = k_stride;
+  p.k_out_stride = k_out_stride;
+  p.v_stride = v_stride;
+  p.Hq = num_q_heads;
+  p.Hkv = (int)c->cfg.num_kv_heads;
+  p.D = (int)c->cfg.head_size;
+  p.bs_log = 4 + c->bs_shift;
+  p.num_blocks = c->cfg.num_blocks;
+  p.eps = eps;
+  p.k_scale = c->fp8 ? c->k_scale[layer] : 1.f;
+  p.v_scale = c->fp8 ? c->v_scale[layer] : 1.f;
+  p.err = c->err_dev;
+  p.special = c->fp8_special();
+  p.rope = rope->table;
+  DeviceGuard g(c->device);
+  PA_CUDA(pa::launch_rope_norm_cache(p, c->cfg.dtype == 0, c->fp8, c->num_sms,
+                                     static_cast<cudaStream_t>(cuda_stream)));
+  return PA_OK;
+}
+
+pa_status pa_gather_cache(PagedAttnCache *c, uint32_t layer, void *key, void *value,
+                          const int32_t *block_tables, const int32_t *starts_host,
+                          const int32_t *cu_lens_host, int32_t num_seqs, int32_t max_blocks_per_seq,
+                          int64_t key_stride, int64_t value_stride, void *cuda_stream) {
+  pa_status st = check_layer(c, layer);
+  if (st != PA_OK) return st;
+  if (num_seqs < 0) return fail(PA_ERR_INVALID_ARG, "num_seqs < 0");
+  if (num_seqs == 0) return PA_OK;
+  if (pa::ArgError e = pa::check_gather_args(c->cfg, key, value, block_tables, starts_host, cu_lens_host, num_seqs,
+                                             max_blocks_per_seq, key_stride, value_stride))
+    return arg_fail(e);
+  pa::GatherParams p{};
+  p.k_pool = c->k[layer];
+  p.v_pool = c->v[layer];
+  p.key = static_cast<pa::elem16 *>(key);
+  p.value = static_cast<pa::elem16 *>(value);
+  p.key_stride = key_stride;
+  p.value_stride = value_stride;
+  p.Hkv = (int)c->cfg.num_kv_heads;
+  p.D = (int)c->cfg.head_size;
+  p.MB = max_blocks_per_seq;
+  p.bs_log = 4 + c->bs_shift;
+  p.num_blocks = c->cfg.num_blocks;
+  p.k_scale = c->fp8 ? c->k_scale[layer] : 1.f;
+  p.v_scale = c->fp8 ? c->v_scale[layer] : 1.f;
+  p.err = c->err_dev;
+  DeviceGuard g(c->device);
+  for (int32_t s0 = 0; s0 < num_seqs; s0 += pa::kMaxPlanSeqs) {
+    p.S = std::min(num_seqs - s0, pa::kMaxPlanSeqs);
+    p.block_tables = block_tables + (int64_t)s0 * max_blocks_per_seq;
+    p.units[0] = 0;
+    for (int i = 0; i < p.S; i++) {
+      const int32_t first = starts_host ? starts_host[s0 + i] : 0, len = cu_lens_host[s0 + i + 1] - cu_lens_host[s0 + i];
+      p.start[i] = first;
+      p.cu[i] = cu_lens_host[s0 + i];
+      const int64_t units = len > 0 ? (((int64_t)first + len + 15) >> 4) - (first >> 4) : 0;
+      p.units[i + 1] = p.units[i] + (int32_t)units;
+    }
+    p.cu[p.S] = cu_lens_host[s0 + p.S];
+    PA_CUDA(pa::launch_gather_cache(p, c->cfg.dtype == 0, c->fp8, static_cast<cudaStream_t>(cuda_stream)));
+  }
+  return PA_OK;
+}
+
+size_t pa_prompt_workspace_bytes(const PagedAttnCache *c) {
+  return c ? pa::prompt_workspace_bytes(c->num_sms, (int)c->cfg.head_size) : 0;
+}
+
+pa_status pa_prompt_attention(PagedAttnCache *c, void *out, const void *q, const void *k, const void *v,
+                              const int32_t *cu_q_lens_host, const int32_t *cu_kv_lens_host,
+                              int32_t num_seqs, int32_t num_q_heads, int64_t q_stride, int64_t k_stride,
+                              int64_t v_stride, int64_t out_stride, float scale, float softcap,
+                              void *workspace, size_t workspace_bytes, void *cuda_stream) {
+  if (!c) return fail(PA_ERR_INVALID_ARG, "cache is null");
+  if (num_seqs < 0) return fail(PA_ERR_INVALID_ARG, "num_seqs < 0");
+  if (num_seqs == 0) return PA_OK;
+  if (pa::ArgError e = pa::check_prompt_args(c->cfg, out, q, k, v, cu_q_lens_host, cu_kv_lens_host, num_seqs,
+                                             num_q_heads, q_stride, k_stride, v_stride, out_stride, scale,
+                                             softcap, workspace, workspace_bytes, pa_prompt_workspace_bytes(c)))
+    return arg_fail(e);
+  const int32_t *cu_kv = cu_kv_lens_host ? cu_kv_lens_host : cu_q_lens_host;
+  pa::PromptParams p{};
+  p.out = static_cast<pa::elem16 *>(out);
+  p.q = static_cast<const pa::elem16 *>(q);
+  p.k = static_cast<const pa::elem16 *>(k);
+  p.v = static_cast<const pa::elem16 *>(v);
+  p.q_stride = q_stride;
+  p.k_stride = k_stride;
+  p.v_stride = v_stride;
+  p.out_stride = out_stride;
+  p.Hq = num_q_heads;
+  p.Hkv = (int)c->cfg.num_kv_heads;
+  p.G = p.Hq / p.Hkv;
+  p.D = (int)c->cfg.head_size;
+  p.scale = scale;
+  p.softcap = softcap;
+  DeviceGuard g(c->device);
+  for (int32_t s0 = 0; s0 < num_seqs; s0 += pa::kMaxPlanSeqs) {
+    p.S = std::min(num_seqs - s0, pa::kMaxPlanSeqs);
+    std::copy(cu_q_lens_host + s0, cu_q_lens_host + s0 + p.S + 1, p.cu_q);
+    std::copy(cu_kv + s0, cu_kv + s0 + p.S + 1, p.cu_kv);
+    try {
+      PA_CUDA(pa::launch_prompt_attention(p, c->cfg.dtype == 0, c->num_sms, workspace, c->err_dev,
+                                          static_cast<cudaStream_t>(cuda_stream)));
+    } catch (const std::bad_alloc &) {
+      return fail(PA_ERR_OOM, "host allocation failed");
+    }
+  }
   return PA_OK;
 }
 

@@ -172,6 +172,60 @@ __device__ __forceinline__ void fp8x4_to_f16(uint32_t w, uint32_t &lo, uint32_t 
 }
 constexpr float kFp8Unbias = 256.f;  // the factor the conversion above leaves out
 
+// ---- 16-bit elements -> FP8 (E4M3) cache bytes -----------------------------------
+// Encoder of the reference's byte format, crates/mlx-paged-attn/metal/float8.metal:63-121:
+// bias 7, exponent field 15 is infinity / NaN (largest finite value 240).  Normal range:
+// round to nearest even, overflow to the infinity code.  Below it: magnitudes under 2^-9
+// become zero, the rest round half up, and a
+// value that would round up to the smallest normal number comes out as zero (the result is
+// masked to the three mantissa bits).  Inputs of magnitude 256 and above miss the normal
+// range test and take the below-normal branch as well; for magnitudes below 16384 that
+// yields the low three bits of a shifted mantissa, which is kept as is so that the bytes
+// match; above, where the reference's shift count turns negative, the infinity code.
+__device__ __forceinline__ uint32_t fp8_e4m3_encode_ref(float f) {
+  const uint32_t bits = __float_as_uint(f);
+  const uint32_t s = (bits >> 31) << 7, a = bits & 0x7FFFFFFFu;
+  if (a >= 0x7F800000u) return s | 0x78u | (a != 0x7F800000u);
+  const int e8 = (int)(a >> 23) - 120;
+  const uint32_t m = a & 0x7FFFFFu;
+  if (e8 >= 1 && e8 <= 14) {
+    uint32_t mant = m >> 20;
+    mant += ((m >> 19) & 1u) & (((m & 0x7FFFFu) != 0u) | (mant & 1u));
+    uint32_t e = (uint32_t)e8;
+    if (mant >> 3) {
+      mant = 0;
+      if (++e > 14u) return s | 0x78u;
+    }
+    return s | (e << 3) | mant;
+  }
+  if (e8 < -2) return s;
+  const int rshift = 21 - e8;
+  if (rshift < 1) return s | 0x78u;
+  return s | ((((0x800000u | m) + (1u << (rshift - 1))) >> rshift) & 7u);
+}
+
+// Eight 16-bit elements (one uint4) -> eight bytes: x / scale in fp32 (IEEE division),
+// rounded to the input type, then encoded
+// (crates/mlx-paged-attn/metal/cache/reshape_and_cache.metal:88-92).
+template <bool F16>
+__device__ __forceinline__ uint2 quantise8(uint4 v, float scale) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t out[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t bits16 = (w[i >> 1] >> ((i & 1) * 16)) & 0xffffu;
+    float x;
+    if (F16) asm("cvt.f32.f16 %0, %1;" : "=f"(x) : "h"((uint16_t)bits16));
+    else x = __uint_as_float(bits16 << 16);
+    const uint32_t r16 = to_elem<F16>(__fdiv_rn(x, scale));
+    float y;
+    if (F16) asm("cvt.f32.f16 %0, %1;" : "=f"(y) : "h"((uint16_t)r16));
+    else y = __uint_as_float(r16 << 16);
+    out[i >> 2] |= fp8_e4m3_encode_ref(y) << ((i & 3) * 8);
+  }
+  return make_uint2(out[0], out[1]);
+}
+
 __device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t w) {
   return pack2<true>(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }

@@ -40,13 +40,24 @@ EXPORTED_SYMBOLS = [
     "pa_swap_in", "pa_swap_block_bytes",
     "pa_decode_step_host", "pa_kernel_launch_count", "pa_decode_step", "pa_varlen_step_host",
     "pa_cache_check_errors_fast", "pa_paged_attention_decode_rows", "pa_decode_step_rows",
+    "pa_rope_create", "pa_rope_free", "pa_rope_frequencies", "pa_rope_norm_and_cache", "pa_gather_cache",
+    "pa_prompt_workspace_bytes", "pa_prompt_attention",
 ]
+
+ROPE_SCALINGS = ("none", "linear", "bands", "yarn")
 
 
 class PagedAttnConfig(C.Structure):
     """Same six u32 fields as crates/mlx-sys/src/lib.rs:690-705."""
     _fields_ = [("block_size", C.c_uint32), ("num_blocks", C.c_uint32), ("head_size", C.c_uint32),
                 ("num_kv_heads", C.c_uint32), ("num_layers", C.c_uint32), ("dtype", C.c_uint32)]
+
+
+class PaRopeConfig(C.Structure):
+    _fields_ = [("rope_dims", C.c_uint32), ("interleaved", C.c_uint32), ("base", C.c_float),
+                ("scaling", C.c_uint32), ("factor", C.c_float), ("original_max_position", C.c_uint32),
+                ("low_freq_factor", C.c_float), ("high_freq_factor", C.c_float),
+                ("beta_fast", C.c_float), ("beta_slow", C.c_float), ("attention_factor", C.c_float)]
 
 
 class PagedAttnError(RuntimeError):
@@ -127,6 +138,16 @@ def load_library() -> C.CDLL:
     lib.pa_varlen_step_host.argtypes = [vp, u32, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, f32, f32]
     lib.pa_decode_step.argtypes = [vp, u32, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i64, i64, i64,
                                    i64, f32, f32, vp, sz, vp]
+    lib.pa_rope_create.argtypes = [C.POINTER(PaRopeConfig), C.POINTER(vp)]
+    lib.pa_rope_free.argtypes = [vp]
+    lib.pa_rope_frequencies.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(f32)]
+    lib.pa_rope_norm_and_cache.argtypes = [vp, u32, vp, vp, vp, vp, vp, vp, vp, vp, f32, vp, vp, i64, i32,
+                                           i64, i64, i64, i64, i64, vp]
+    lib.pa_gather_cache.argtypes = [vp, u32, vp, vp, vp, vp, vp, i32, i32, i64, i64, vp]
+    lib.pa_prompt_workspace_bytes.argtypes = [vp]
+    lib.pa_prompt_workspace_bytes.restype = sz
+    lib.pa_prompt_attention.argtypes = [vp, vp, vp, vp, vp, vp, vp, i32, i32, i64, i64, i64, i64, f32, f32,
+                                        vp, sz, vp]
     # tier 1
     lib.mlx_paged_attn_create_cache.argtypes = [C.POINTER(PagedAttnConfig)]
     lib.mlx_paged_attn_create_cache.restype = vp
@@ -182,6 +203,35 @@ def _ptr(x) -> int:
 
 def kernel_launch_count() -> int:
     return int(load_library().pa_kernel_launch_count())
+
+
+class RopePlan:
+    """Owner of a PaRope plan: which elements of a head rotate, in which pairs, how fast."""
+
+    def __init__(self, rope_dims: int, base: float, interleaved: bool = False, scaling: str = "none",
+                 factor: float = 1.0, original_max_position: int = 0, low_freq_factor: float = 1.0,
+                 high_freq_factor: float = 4.0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 attention_factor: float = 0.0):
+        self.lib = load_library()
+        self.handle = C.c_void_p()
+        if scaling not in ROPE_SCALINGS:
+            raise ValueError(f"scaling must be one of {ROPE_SCALINGS}")
+        self.cfg = PaRopeConfig(rope_dims, int(interleaved), base, ROPE_SCALINGS.index(scaling), factor,
+                                original_max_position, low_freq_factor, high_freq_factor, beta_fast,
+                                beta_slow, attention_factor)
+        _check(self.lib.pa_rope_create(C.byref(self.cfg), C.byref(self.handle)))
+
+    def __del__(self):
+        try:
+            self.lib.pa_rope_free(self.handle)
+        except Exception:
+            pass
+
+    def frequencies(self):
+        """(radians per position of every pair, gain of sine and cosine)."""
+        f, g = (C.c_double * (self.cfg.rope_dims // 2))(), C.c_float()
+        _check(self.lib.pa_rope_frequencies(self.handle, f, C.byref(g)))
+        return list(f), g.value
 
 
 class PagedCache:
@@ -275,6 +325,46 @@ class PagedCache:
             _ptr(k_norm_weight) if k_norm_weight is not None else None, eps, _ptr(positions),
             rope_base, rope_dims, _ptr(slot_mapping), num_tokens, num_q_heads, q_stride,
             q_out_stride, k_stride, v_stride, stream))
+
+    def rope_norm_and_cache(self, rope: "RopePlan", q_out, k_out, q, k, v, q_norm_weight, k_norm_weight,
+                            eps: float, positions, slot_mapping, num_tokens: int, num_q_heads: int,
+                            q_stride: int | None = None, q_out_stride: int | None = None,
+                            k_stride: int | None = None, k_out_stride: int | None = None,
+                            v_stride: int | None = None, layer: int = 0, stream: int = 0) -> None:
+        """Head norms, rotation by a plan and KV write in one launch (k_out, weights and
+        slot_mapping may be None)."""
+        q_row, kv_row = num_q_heads * self.cfg.head_size, self.cfg.num_kv_heads * self.cfg.head_size
+        _check(self.lib.pa_rope_norm_and_cache(
+            self.handle, layer, rope.handle, _ptr(q_out), _ptr(k_out), _ptr(q), _ptr(k), _ptr(v),
+            _ptr(q_norm_weight), _ptr(k_norm_weight), eps, _ptr(positions), _ptr(slot_mapping),
+            num_tokens, num_q_heads, q_stride or q_row, q_out_stride or q_row, k_stride or kv_row,
+            k_out_stride or kv_row, v_stride or kv_row, stream))
+
+    def gather(self, key, value, block_tables, starts_host, cu_lens_host, num_seqs: int,
+               max_blocks_per_seq: int, key_stride: int | None = None,
+               value_stride: int | None = None, layer: int = 0, stream: int = 0) -> None:
+        """Cached keys and values of token ranges as packed rows (starts_host may be None)."""
+        row = self.cfg.num_kv_heads * self.cfg.head_size
+        _check(self.lib.pa_gather_cache(
+            self.handle, layer, _ptr(key), _ptr(value), _ptr(block_tables), _ptr(starts_host),
+            _ptr(cu_lens_host), num_seqs, max_blocks_per_seq, key_stride or row, value_stride or row,
+            stream))
+
+    def prompt_workspace_bytes(self) -> int:
+        return int(self.lib.pa_prompt_workspace_bytes(self.handle))
+
+    def prompt_attention(self, out, q, k, v, cu_q_lens_host, cu_kv_lens_host, num_seqs: int,
+                         num_q_heads: int, scale: float, workspace, workspace_bytes: int,
+                         softcap: float = 1.0, q_stride: int | None = None,
+                         k_stride: int | None = None, v_stride: int | None = None,
+                         out_stride: int | None = None, stream: int = 0) -> None:
+        """Causal attention of packed prompts over contiguous keys and values."""
+        q_row, kv_row = num_q_heads * self.cfg.head_size, self.cfg.num_kv_heads * self.cfg.head_size
+        _check(self.lib.pa_prompt_attention(
+            self.handle, _ptr(out), _ptr(q), _ptr(k), _ptr(v), _ptr(cu_q_lens_host),
+            _ptr(cu_kv_lens_host), num_seqs, num_q_heads, q_stride or q_row, k_stride or kv_row,
+            v_stride or kv_row, out_stride or q_row, scale, softcap, _ptr(workspace), workspace_bytes,
+            stream))
 
     def copy_blocks(self, block_mapping, num_pairs: int, layer: int = 0, stream: int = 0) -> None:
         _check(self.lib.pa_copy_blocks(self.handle, layer, _ptr(block_mapping), num_pairs, stream))
