@@ -1,18 +1,175 @@
-// Causal attention of packed prompts over contiguous keys and values.
+// Causal attention of packed prompts over contiguous keys and values: tcgen05 tensor cores,
+// accumulators in TMEM, every operand brought in by tensor-map copies, sm_100a.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i k_j - m_i),  j <= kv_len - q_len + i
+//
+// with m_i any number near the row's largest logit (it cancels).  One pass over the keys: the
+// running maximum and sum are kept in fp32 per row; the maximum is stale - it moves only when
+// a logit exceeds it by more than 2^8 - so that the accumulator is rarely rescaled.
+// Probabilities are rounded to the 16-bit type because the tensor cores take both operands of
+// P.V in one 16-bit type; their sum is taken before the rounding.
+//
+// Work: an item is up to 256 rows of one (sequence, kv head), a row being a (query token, head
+// of the group) pair, so that every key tile is read once for the whole group: two 128-row
+// query tiles that share each 128-key tile (head sizes above 128: one query tile, the
+// accumulator takes all the columns two would).  The line of items is cut into one piece of
+// equal cost per CTA (plan_prompt); an item that a cut splits leaves fp32 partial results in
+// the workspace, joined in CTA order by prompt_join_kernel, so that few rows over long keys
+// use every SM and the same call gives the same bits.
+//
+// Roles (warps):
+//   8 per query tile  softmax: two threads per row, each 64 of a tile's 128 logits, so that a
+//                     scheduler has two warps of a tile in flight while the other query tile
+//                     is in the tensor cores
+//   1                 copies: Q per item, K and V tiles into two rings
+//   1                 issues every tcgen05.mma (two more idle: register budgets move between
+//                     warpgroups of four)
+// TMEM (512 columns): logits S0 | S1 (128 each), outputs O0 | O1.  P overwrites the first half
+// of the thread's own logit columns and is the A operand of O += P.V.
+// K tiles and Q are K-major with the 128-byte swizzle; a V tile lands the same way - rows of
+// tokens - and is read as an MN-major B operand, so nothing is transposed on the way.
+//
+// S_i(j+1) overwrites P_i(j), and the tensor cores order only MMAs of one accumulator and
+// shape, so it is issued after P_i(j).V(j) has signalled completion; the other query tile's
+// work fills the pipe meanwhile.
+//
+// A probability of a masked key is exactly 0, but 0 * NaN is NaN: a row whose result is not
+// finite is checked for masked values that are not, and then recomputed by itself over the keys
+// that it sees (repair_row).  The check costs a comparison per output element.
+//
+// Every wait is bounded; on expiry the CTA raises the error word, every role leaves its loop,
+// copies in flight are drained and TMEM is freed.
+#include <cuda.h>
+
 #include "prompt_path.cuh"
+#include "tile_common.cuh"
 
 namespace pa {
 
 namespace {
 
-// One row - a (query token, query head) - by one warp: 32 keys at a time, a lane per key for
-// the logits, the online softmax across the warp, then a lane per D/32 output dimensions.
+using namespace tile;
+
+constexpr int kBox = 128 * 128;  // one operand slab: 128 rows x 64 elements
+
+template <int NBOX>
+struct Geo {
+  static constexpr int QT = NBOX <= 2 ? 2 : 1;          // query tiles of an item
+  static constexpr int NK = NBOX == 1 ? 5 : NBOX <= 3 ? 2 : 1;  // ring depths, tiles of NBOX slabs
+  static constexpr int NV = NBOX == 1 ? 5 : NBOX == 2 ? 2 : 1;
+  static constexpr int kTile = NBOX * kBox;
+  static constexpr int kSoft = 8 * QT;                  // softmax warps
+  static constexpr int kThreads = (kSoft + 4) * 32;     // whole warpgroups
+  static constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK,
+                       B_VEMPTY = B_VFULL + NV, B_SFULL = B_VEMPTY + NV, B_PREADY = B_SFULL + QT,
+                       B_PVDONE = B_PREADY + QT, kBars = B_PVDONE + QT;
+  static constexpr int kXch = 2 * QT * 2 * 128 * 4;     // [parity][query tile][half][row] floats
+  static constexpr int kWalk = kThreads / 32 * 16;       // a PlanPos per warp
+  static constexpr int kSmem = 1024 + (QT + NK + NV) * kTile + kXch + kWalk + kBars * 8 + 16;
+  static_assert(kSmem <= 232448, "shared memory per CTA");
+};
+
+struct PromptLaunch {
+  PromptParams p;
+  PlanPos begin[kMaxPlanCtas + 1];
+  float *ws;       // two partial slots per CTA, each [D + 2][128 * QT] floats
+  unsigned *err;
+  int32_t sub_tokens, tile_tokens;
+};
+
+// Where a CTA is on the line of items; every role walks it for itself.
+struct Seg {
+  int s, h, qt, kt0, kt1, n;  // key tiles [kt0, kt1) of the item's n
+  int q_len, kv_len, q0, tiles;
+};
+// The position lives in shared memory, one per warp: it is touched once per item and would
+// otherwise hold registers through the softmax.
+template <bool WARP>  // a whole warp walks, or one lane
+__device__ __forceinline__ bool walk_next(const PromptLaunch &L, PlanPos *at, Seg &g) {
+  if (WARP) __syncwarp();
+  struct {
+    PlanPos p, e;
+  } w = {*at, L.begin[blockIdx.x + 1]};
+  if (w.p.seq == w.e.seq && w.p.head == w.e.head && w.p.qt == w.e.qt && w.p.kt >= w.e.kt) return false;
+  g.s = w.p.seq;
+  g.h = w.p.head;
+  g.qt = w.p.qt;
+  g.q_len = L.p.cu_q[g.s + 1] - L.p.cu_q[g.s];
+  g.kv_len = L.p.cu_kv[g.s + 1] - L.p.cu_kv[g.s];
+  g.q0 = g.qt * L.tile_tokens;
+  const int q1 = min(g.q_len, g.q0 + L.tile_tokens);
+  g.tiles = q1 - g.q0 > L.sub_tokens ? 2 : 1;
+  const int keys = max(g.kv_len - g.q_len + q1, 0);
+  g.n = (keys + kKeyTile - 1) / kKeyTile;
+  g.kt0 = w.p.kt;
+  const bool cut = w.e.seq == g.s && w.e.head == g.h && w.e.qt == g.qt;
+  g.kt1 = cut ? w.e.kt : g.n;
+  w.p.kt = 0;
+  if (cut) {
+    w.p = w.e;
+  } else if (q1 < g.q_len) {
+    w.p.qt++;
+  } else {
+    w.p.qt = 0;
+    if (++w.p.head == L.p.Hkv) {
+      w.p.head = 0;
+      for (w.p.seq++; w.p.seq < L.p.S && L.p.cu_q[w.p.seq + 1] == L.p.cu_q[w.p.seq];) w.p.seq++;
+    }
+  }
+  if (WARP) __syncwarp();  // every lane has read it
+  *at = w.p;
+  return true;
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
+                 "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// V tile as the B operand of P.V, N (head dimension) contiguous: 128-byte swizzle, slabs of 64
+// dimensions kBox apart (leading byte offset), groups of 8 tokens 1024 B apart (stride).
+__device__ __forceinline__ uint64_t v_mn_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(kBox >> 4) << 16) | (64ull << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+// fp32 accumulator, M = 128; bit 16: B is MN-major
+__device__ __forceinline__ uint32_t mma_desc(bool f16, uint32_t n, bool b_mn) {
+  return (1u << 4) | (f16 ? 0u : ((1u << 7) | (1u << 10))) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// One row - a (query token, query head) - by one warp over exactly the keys it sees: 32 keys
+// at a time, a lane per key for the logits, the online softmax across the warp, then a lane per
+// output dimension.  Writes the 8-column pieces whose bit is set in `pieces`.
 template <bool F16>
-__device__ void attend_row(const PromptParams &p, int s, int token, int head, elem16 *out) {
+__device__ __noinline__ void repair_row(const PromptParams &p, int s, int token, int head, uint32_t pieces) {
   const int lane = threadIdx.x & 31, D = p.D, h = head / p.G;
   const int q_len = p.cu_q[s + 1] - p.cu_q[s], kv_len = p.cu_kv[s + 1] - p.cu_kv[s];
   const int keys = kv_len - q_len + token + 1;
   const elem16 *q = p.q + (int64_t)(p.cu_q[s] + token) * p.q_stride + (int64_t)head * D;
+  elem16 *out = p.out + (int64_t)(p.cu_q[s] + token) * p.out_stride + (int64_t)head * D;
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
   for (int j0 = 0; j0 < keys; j0 += 32) {
     const int j = j0 + lane;
@@ -51,25 +208,482 @@ __device__ void attend_row(const PromptParams &p, int s, int token, int head, el
         if (i * 32 + lane < D) o[i] = fmaf(wj, elem_value<F16>(v[i * 32 + lane]), o[i]);
     }
   }
-  const float inv = keys > 0 ? 1.f / l : 0.f;
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // no key: zeros; NaN stays
 #pragma unroll
   for (int i = 0; i < 8; i++)
-    if (i * 32 + lane < D) out[i * 32 + lane] = to_elem<F16>(keys > 0 ? o[i] * inv : 0.f);
+    if (i * 32 + lane < D && (pieces >> (i * 4 + (lane >> 3)) & 1u)) out[i * 32 + lane] = to_elem<F16>(o[i] * inv);
 }
 
-template <bool F16>
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const PromptParams p) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int64_t total = (int64_t)(p.cu_q[p.S] - p.cu_q[0]) * p.Hq;
-  if (row >= total) return;
-  const int t = p.cu_q[0] + (int)(row / p.Hq), head = (int)(row % p.Hq);
-  int lo = 0, hi = p.S;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_q[mid] <= t) lo = mid;
-    else hi = mid;
+// Whether a value outside the keys that a row sees, but inside the key tiles that its item
+// reads, is not finite (the tiles run on into the rows of the next sequences).
+__device__ __noinline__ bool masked_value_not_finite(const PromptParams &p, int s, int token, int h, int n_tiles, bool f16) {
+  const int lane = threadIdx.x & 31;
+  const int q_len = p.cu_q[s + 1] - p.cu_q[s], kv_len = p.cu_kv[s + 1] - p.cu_kv[s];
+  const int first = max(kv_len - q_len + token + 1, 0);
+  const int64_t end = min((int64_t)n_tiles * kKeyTile, (int64_t)p.cu_kv[p.S] - p.cu_kv[s]);
+  const uint32_t top = f16 ? 0x7C00u : 0x7F80u;  // the exponent of infinity and NaN
+  bool bad = false;
+  for (int64_t j = first; j < end; j++) {
+    const elem16 *v = p.v + (p.cu_kv[s] + j) * p.v_stride + (int64_t)h * p.D;
+    for (int d = lane; d < p.D; d += 32) bad |= (v[d] & top) == top;
   }
-  attend_row<F16>(p, lo, t - p.cu_q[lo], head, p.out + (int64_t)t * p.out_stride + (int64_t)head * p.D);
+  return __any_sync(0xffffffffu, bad);
+}
+
+template <int NBOX, bool CAP, bool F16>
+__global__ void __launch_bounds__(Geo<NBOX>::kThreads, 1)
+prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_constant__ CUtensorMap q_map,
+                        const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+  using Z = Geo<NBOX>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t q_s = base, k_s = q_s + Z::QT * Z::kTile, v_s = k_s + Z::NK * Z::kTile;
+  float *xch = reinterpret_cast<float *>(gen + (Z::QT + Z::NK + Z::NV) * Z::kTile);
+  PlanPos *const at = reinterpret_cast<PlanPos *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch) + (threadIdx.x >> 5);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch + Z::kWalk);
+  uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Z::kBars);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  const PromptParams &p = L.p;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int G = p.G, D = p.D;
+  if (tid == 0) {
+    mbar_init(bar(Z::B_QFULL), 1);
+    mbar_init(bar(Z::B_QEMPTY), 1);
+    for (int i = 0; i < Z::NK; i++) mbar_init(bar(Z::B_KFULL + i), 1), mbar_init(bar(Z::B_KEMPTY + i), 1);
+    for (int i = 0; i < Z::NV; i++) mbar_init(bar(Z::B_VFULL + i), 1), mbar_init(bar(Z::B_VEMPTY + i), 1);
+    for (int i = 0; i < Z::QT; i++) {
+      mbar_init(bar(Z::B_SFULL + i), 1);
+      mbar_init(bar(Z::B_PREADY + i), 8);
+      mbar_init(bar(Z::B_PVDONE + i), 1);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == Z::kSoft + 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_holder)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  bool failed = false;
+  Seg g;
+  if (lane == 0) *at = L.begin[blockIdx.x];
+  __syncwarp();
+
+  // Two threads per row and two query tiles make 640 threads of 96 registers; the softmax needs a
+  // few more: 16 warps x 104 + 4 x 56 = 60416 of the 61440 that the launch holds.
+  if (warp >= Z::kSoft) {
+    if (Z::QT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == Z::kSoft) {
+      // =========================== copies ==============================================
+      if (lane == 0) {
+        uint32_t items = 0, tiles = 0;  // items and key tiles fetched so far
+        while (!failed && walk_next<false>(L, at, g)) {
+          if (g.kt0 >= g.kt1) continue;
+          if (items > 0 && !wait_bar(bar(Z::B_QEMPTY), (items - 1) & 1, abort_flag)) { failed = true; break; }
+          mbar_expect_tx(bar(Z::B_QFULL), (uint32_t)(g.tiles * NBOX * L.sub_tokens * G) * 128u);
+          for (int i = 0; i < g.tiles; i++)
+            for (int b = 0; b < NBOX; b++)
+              tma_load_3d(q_s + (i * NBOX + b) * kBox, &q_map, b * 64, g.h * G, p.cu_q[g.s] + g.q0 + i * L.sub_tokens,
+                          bar(Z::B_QFULL));
+          items++;
+          for (int t = g.kt0; t < g.kt1; t++, tiles++) {
+            const int row = p.cu_kv[g.s] + t * kKeyTile;
+            const int ks = tiles % Z::NK, vs = tiles % Z::NV;
+            if (tiles >= Z::NK && !wait_bar(bar(Z::B_KEMPTY + ks), (tiles / Z::NK - 1) & 1, abort_flag)) { failed = true; break; }
+            mbar_expect_tx(bar(Z::B_KFULL + ks), Z::kTile);
+            for (int b = 0; b < NBOX; b++)
+              tma_load_3d(k_s + ks * Z::kTile + b * kBox, &k_map, b * 64, g.h, row, bar(Z::B_KFULL + ks));
+            if (tiles >= Z::NV && !wait_bar(bar(Z::B_VEMPTY + vs), (tiles / Z::NV - 1) & 1, abort_flag)) { failed = true; break; }
+            mbar_expect_tx(bar(Z::B_VFULL + vs), Z::kTile);
+            for (int b = 0; b < NBOX; b++)
+              tma_load_3d(v_s + vs * Z::kTile + b * kBox, &v_map, b * 64, g.h, row, bar(Z::B_VFULL + vs));
+          }
+        }
+      }
+      __syncwarp();
+    } else if (warp == Z::kSoft + 1) {
+      // =========================== MMA issue ===========================================
+      // The whole warp walks the loop so that descriptors and addresses stay warp-uniform; one
+      // elected lane issues.  Its waits end alike for every lane.
+      auto wait_all = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(b, parity, abort_flag)) != 0; };
+      const uint32_t idesc_s = mma_desc(F16, 128, false), idesc_pv = mma_desc(F16, (uint32_t)(D + 15) & ~15u, true);
+      const int ksteps = (D + 15) >> 4;
+      const bool leader = elect_one();
+      uint32_t items = 0, tiles = 0;
+      uint32_t cnt[Z::QT];  // logit tiles issued for each query tile
+#pragma unroll
+      for (int i = 0; i < Z::QT; i++) cnt[i] = 0;
+      auto issue_s = [&](int i, uint32_t t) {
+        const uint32_t kst = k_s + (t % Z::NK) * Z::kTile;
+#pragma unroll
+        for (int kk = 0; kk < NBOX * 4; kk++) {
+          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32;
+          if (leader && kk < ksteps)
+            umma_ss(tmem + i * 128, sw128_desc(q_s + i * Z::kTile + off), sw128_desc(kst + off), idesc_s, kk > 0 ? 1u : 0u);
+        }
+        if (leader) tc_commit(bar(Z::B_SFULL + i));
+      };
+      auto issue_pv = [&](int i, uint32_t t, bool first) {
+        const uint32_t vst = v_s + (t % Z::NV) * Z::kTile;
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++)
+          if (leader)
+            umma_ts(tmem + 256 + i * 128, tmem + i * 128 + (kk >> 2) * 64 + (kk & 3) * 8, v_mn_desc(vst + kk * 2048), idesc_pv,
+                    first && kk == 0 ? 0u : 1u);
+        if (leader) tc_commit(bar(Z::B_PVDONE + i));
+      };
+      // S_i of key tile t into its buffer, once P_i.V of the tile before it is through with it
+      auto next_s = [&](int i, uint32_t t) {
+        if (cnt[i] > 0 && !wait_all(bar(Z::B_PVDONE + i), (cnt[i] - 1) & 1)) return false;
+        tc_fence_after();
+        issue_s(i, t);
+        cnt[i]++;
+        return true;
+      };
+      while (!failed && walk_next<true>(L, at, g)) {
+        const int n = g.kt1 - g.kt0;
+        if (n <= 0) continue;
+        if (!wait_all(bar(Z::B_QFULL), items & 1) ||
+            !wait_all(bar(Z::B_KFULL + tiles % Z::NK), (tiles / Z::NK) & 1)) { failed = true; break; }
+#pragma unroll
+        for (int i = 0; i < Z::QT; i++)
+          if (i < g.tiles && !failed) failed = !next_s(i, tiles);
+        if (failed) break;
+        if (leader) {
+          tc_commit(bar(Z::B_KEMPTY + tiles % Z::NK));
+          if (n == 1) tc_commit(bar(Z::B_QEMPTY));
+        }
+        for (int j = 0; j < n && !failed; j++) {
+          const uint32_t t = tiles + j;
+          if (!wait_all(bar(Z::B_VFULL + t % Z::NV), (t / Z::NV) & 1)) { failed = true; break; }
+#pragma unroll
+          for (int i = 0; i < Z::QT; i++) {
+            if (i >= g.tiles || failed) continue;
+            if (!wait_all(bar(Z::B_PREADY + i), (cnt[i] - 1) & 1)) { failed = true; continue; }
+            tc_fence_after();
+            issue_pv(i, t, j == 0);
+            const bool last = i + 1 == g.tiles;
+            if (last && leader) tc_commit(bar(Z::B_VEMPTY + t % Z::NV));
+            if (j + 1 < n) {
+              if (i == 0 && !wait_all(bar(Z::B_KFULL + (t + 1) % Z::NK), ((t + 1) / Z::NK) & 1)) { failed = true; continue; }
+              if (!next_s(i, t + 1)) { failed = true; continue; }
+              if (last && leader) {
+                tc_commit(bar(Z::B_KEMPTY + (t + 1) % Z::NK));
+                if (j + 2 == n) tc_commit(bar(Z::B_QEMPTY));
+              }
+            }
+          }
+          __syncwarp();
+        }
+        tiles += n;
+        items++;
+      }
+    }
+  } else {
+    // =========================== softmax + epilogue ==================================
+    if (Z::QT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    const int i = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3;
+    const int row = quad * 32 + lane;  // row of the query tile = TMEM lane
+    const int tok_in = row / G, head_in = row - tok_in * G;
+    const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
+    const uint32_t s_t = tmem + lane_base + i * 128 + half * 64;
+    const uint32_t o_t = tmem + lane_base + 256 + i * 128;
+    const int sync_id = 1 + i * 4 + quad;  // the two warps that share these rows
+    const uint32_t mine = smem_u32(xch) + ((i * 2 + half) * 128 + row) * 4;
+    uint32_t xc = 0;   // exchanges so far: two slots in turn
+    uint32_t cnt = 0;  // logit tiles seen
+    const float c = p.scale * kLog2e;
+    // soft-capping: x -> tanh(x*scale/cap)*cap/scale, so that x*c is the capped logit
+    const float cap_in = p.scale / p.softcap, cap_out = p.softcap / p.scale;
+    auto exchange = [&](float x) {
+      const uint32_t a = mine + (xc++ & 1) * (Z::QT * 2 * 128 * 4), b = a + (half ? -512 : 512);
+      float y;
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory");
+      pair_sync(sync_id);
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(b) : "memory");
+      return y;
+    };
+    // After a wait that ran out these warps keep going through the motions (every further wait
+    // returns at once): two of them share each row's barrier, and one that left would leave
+    // the other waiting at it.
+    while (walk_next<true>(L, at, g)) {
+      if (i >= g.tiles) continue;
+      const int token = g.q0 + i * L.sub_tokens + tok_in;  // within the sequence
+      const bool valid = tok_in < L.sub_tokens && token < g.q_len;
+      const int lim = valid ? g.kv_len - g.q_len + token + 1 : 0x7fffffff;  // keys the row sees
+      int min_lim = lim;
+#pragma unroll
+      for (int o = 16; o >= 1; o >>= 1) min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, o));
+      float m_used = -INFINITY, l = 0.f;
+      for (int t = g.kt0; t < g.kt1; t++, cnt++) {
+        failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
+        __syncwarp();
+        tc_fence_after();
+        const int key0 = t * kKeyTile + half * 64;
+        const bool need_mask = key0 + 64 > min_lim;
+        const int left = lim - key0;  // columns from here on are masked
+        auto cap_and_mask = [&](uint32_t (&r)[16], int col0) {
+          if (CAP) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) r[e] = __float_as_uint(tanhf(__uint_as_float(r[e]) * cap_in) * cap_out);
+          }
+          if (need_mask) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+              if (col0 + e >= left) r[e] = 0xff800000u;
+          }
+        };
+        float mx, sum;
+        uint32_t pr[32];  // the row half's probabilities, packed
+        bool settled = t == g.kt0;
+        if (settled) {  // the first tile sets the reference
+          mx = -INFINITY;
+#pragma unroll
+          for (int ch = 0; ch < 4; ch++) {
+            uint32_t r[16];
+            tmem_ld16(s_t + ch * 16, r);
+            tmem_wait_ld16(r);
+            cap_and_mask(r, ch * 16);
+#pragma unroll
+            for (int e = 0; e < 16; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
+          }
+          m_used = fmaxf(mx, exchange(mx));
+        }
+        for (;;) {
+          const float mc = m_used == -INFINITY ? 0.f : m_used * c;
+          float mxa[2] = {-INFINITY, -INFINITY}, sma[4] = {0.f, 0.f, 0.f, 0.f};
+          // 16 columns at a time, the next 16 on their way from TMEM meanwhile
+          uint32_t a[16], b[16];
+          auto part_pass = [&](uint32_t (&r)[16], int ch) {
+            cap_and_mask(r, ch * 16);
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float x0 = __uint_as_float(r[e]), x1 = __uint_as_float(r[e + 1]);
+              mxa[(e >> 1) & 1] = fmaxf(mxa[(e >> 1) & 1], fmaxf(x0, x1));
+              const float p0 = fast_exp2(fmaf(x0, c, -mc)), p1 = fast_exp2(fmaf(x1, c, -mc));
+              sma[e & 2] += p0;
+              sma[(e & 2) + 1] += p1;
+              pr[ch * 8 + (e >> 1)] = pack2<F16>(p0, p1);
+            }
+          };
+          tmem_ld16(s_t, a);
+          tmem_wait_ld16(a);
+          tmem_ld16(s_t + 16, b);
+          part_pass(a, 0);
+          tmem_wait_ld16(b);
+          tmem_ld16(s_t + 32, a);
+          part_pass(b, 1);
+          tmem_wait_ld16(a);
+          tmem_ld16(s_t + 48, b);
+          part_pass(a, 2);
+          tmem_wait_ld16(b);
+          part_pass(b, 3);
+          mx = fmaxf(mxa[0], mxa[1]);
+          sum = (sma[0] + sma[1]) + (sma[2] + sma[3]);
+          if (settled) break;
+          // both halves of a row see the same maximum and decide alike
+          mx = fmaxf(mx, exchange(mx));
+          const bool grew = valid && mx > m_used && !((mx - m_used) * c <= 8.f);
+          if (!__any_sync(0xffffffffu, grew)) break;
+          float factor = 1.f;
+          if (grew) {
+            factor = m_used == -INFINITY ? 0.f : fast_exp2((m_used - mx) * c);
+            m_used = mx;
+          }
+          // O holds the tiles before this one: S of this tile was issued after their P.V
+          for (int ch = half; ch * 32 < D; ch += 2) {
+            uint32_t r[32];
+            tmem_ld32(o_t + ch * 32, r);
+            tmem_wait_ld32(r);
+#pragma unroll
+            for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
+            tmem_st32(o_t + ch * 32, r);
+          }
+          l *= factor;
+          settled = true;  // the logits are still in TMEM: once more against the new reference
+        }
+        l += sum;
+        tmem_st32(s_t, pr);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(Z::B_PREADY + i));
+      }
+      const int64_t q_row = p.cu_q[g.s] + token;
+      const bool whole = g.kt0 == 0 && g.kt1 == g.n;
+      elem16 *orow = p.out + q_row * p.out_stride + (int64_t)(g.h * G + head_in) * D;
+      if (g.n == 0) {  // no key for any row of the item
+        if (valid)
+          for (int ch = half; ch * 32 < D; ch += 2)
+            for (int e = ch * 32; e < D && e < ch * 32 + 32; e += 8) *reinterpret_cast<uint4 *>(orow + e) = make_uint4(0, 0, 0, 0);
+        continue;
+      }
+      const float l_other = exchange(l);
+      l = half == 0 ? l + l_other : l_other + l;
+      failed |= !wait_bar(bar(Z::B_PVDONE + i), (cnt - 1) & 1, abort_flag);
+      __syncwarp();
+      tc_fence_after();
+      const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+      constexpr int kRows = 128 * Z::QT;
+      float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 2) * kRows + i * 128 + row;
+      bool finite = true;
+      for (int ch = half; ch * 32 < D; ch += 2) {
+        uint32_t r[32];
+        tmem_ld32(o_t + ch * 32, r);
+        tmem_wait_ld32(r);
+        if (valid && whole) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float y[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) y[k] = __uint_as_float(r[e + k]) * inv;
+            if (ch * 32 + e < D) {
+#pragma unroll
+              for (int k = 0; k < 8; k++) finite &= fabsf(y[k]) < INFINITY;
+              *reinterpret_cast<uint4 *>(orow + ch * 32 + e) =
+                  make_uint4(pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3]), pack2<F16>(y[4], y[5]), pack2<F16>(y[6], y[7]));
+            }
+          }
+        } else if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; e++)
+            if (ch * 32 + e < D) part[(size_t)(ch * 32 + e) * kRows] = __uint_as_float(r[e]);
+        }
+        __syncwarp();
+      }
+      if (!whole && valid && half == 0) {
+        part[(size_t)D * kRows] = m_used == -INFINITY ? -INFINITY : m_used * c;
+        part[(size_t)(D + 1) * kRows] = l;
+      }
+      tc_fence_before();
+      uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite);
+      __syncwarp();
+      while (odd) {
+        const int src = __ffs(odd) - 1;
+        odd &= odd - 1;
+        const int tk = __shfl_sync(0xffffffffu, token, src), hd = g.h * G + __shfl_sync(0xffffffffu, head_in, src);
+        if (masked_value_not_finite(p, g.s, tk, g.h, g.n, F16)) repair_row<F16>(p, g.s, tk, hd, half ? 0xF0F0F0F0u : 0x0F0F0F0Fu);
+      }
+    }
+  }
+
+  if (failed) atomicOr(L.err, kErrTimeout);
+  // ---- teardown -------------------------------------------------------------------
+  // A role that gave up may have left copies in flight towards this CTA's shared memory; the
+  // CTA must not exit before they have landed.
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && warp == Z::kSoft) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < (1ll << 22)) {
+    }  // ~2 ms: far longer than any copy takes; nothing below reads shared memory
+  }
+  __syncthreads();
+  if (warp == Z::kSoft + 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+struct JoinLaunch {
+  PromptParams p;
+  const float *ws;
+  int32_t sub_tokens, tile_tokens, rows;  // rows of a partial slot: 128 per query tile
+  PlanPos item[kMaxPlanCtas];             // .kt unused
+  int32_t first[kMaxPlanCtas], last[kMaxPlanCtas];
+};
+
+// Joins the partial results of the items that were cut: out = sum_c w_c O_c / sum_c w_c l_c with
+// w_c = 2^(m_c - max m), pieces in CTA order.  A warp takes 32 rows and 8 dimensions at a time;
+// partials are stored dimension-major, so that its loads are whole lines.
+template <bool F16>
+__global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ JoinLaunch J) {
+  const PromptParams &p = J.p;
+  const PlanPos it = J.item[blockIdx.x];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.D, G = p.G;
+  const int row = blockIdx.y * 32 + lane;  // 128 per query tile
+  const int tile_i = row >> 7, tok_in = (row & 127) / G, head_in = (row & 127) - tok_in * G;
+  const int q_len = p.cu_q[it.seq + 1] - p.cu_q[it.seq], kv_len = p.cu_kv[it.seq + 1] - p.cu_kv[it.seq];
+  const int q0 = it.qt * J.tile_tokens, token = q0 + tile_i * J.sub_tokens + tok_in;
+  const bool valid = tok_in < J.sub_tokens && token < q_len;
+  if (!__any_sync(0xffffffffu, valid)) return;
+  const int n = (max(kv_len - q_len + min(q_len, q0 + J.tile_tokens), 0) + kKeyTile - 1) / kKeyTile;
+  const int c0 = J.first[blockIdx.x], c1 = J.last[blockIdx.x];
+  const size_t slot = (size_t)(D + 2) * J.rows;
+  // the first piece begins the item: the second slot of its CTA; the others the first
+  auto part = [&](int c) { return J.ws + (size_t)(2 * c + (c == c0 ? 1 : 0)) * slot + row; };
+  float mx = -INFINITY, l = 0.f;
+  for (int c = c0; c <= c1; c++)
+    if (valid) mx = fmaxf(mx, part(c)[(size_t)D * J.rows]);
+  const float base = mx == -INFINITY ? 0.f : mx;
+  for (int c = c0; c <= c1; c++)
+    if (valid) l += fast_exp2(part(c)[(size_t)D * J.rows] - base) * part(c)[(size_t)(D + 1) * J.rows];
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  elem16 *orow = p.out + (int64_t)(p.cu_q[it.seq] + token) * p.out_stride + (int64_t)(it.head * G + head_in) * D;
+  for (int d = warp * 8; d < D; d += 64) {
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int c = c0; c <= c1; c++) {
+      if (!valid) continue;
+      const float m = part(c)[(size_t)D * J.rows];
+      if (m == -INFINITY) continue;  // the row sees no key of this piece
+      const float wgt = fast_exp2(m - base);
+#pragma unroll
+      for (int k = 0; k < 8; k++) o[k] = fmaf(wgt, part(c)[(size_t)(d + k) * J.rows], o[k]);
+    }
+    bool finite = true;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      o[k] *= inv;
+      finite &= fabsf(o[k]) < INFINITY;
+    }
+    if (valid)
+      *reinterpret_cast<uint4 *>(orow + d) =
+          make_uint4(pack2<F16>(o[0], o[1]), pack2<F16>(o[2], o[3]), pack2<F16>(o[4], o[5]), pack2<F16>(o[6], o[7]));
+    uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite);
+    __syncwarp();
+    while (odd) {
+      const int src = __ffs(odd) - 1;
+      odd &= odd - 1;
+      const int tk = __shfl_sync(0xffffffffu, token, src), hd = it.head * G + __shfl_sync(0xffffffffu, head_in, src);
+      if (masked_value_not_finite(p, it.seq, tk, it.head, n, F16)) repair_row<F16>(p, it.seq, tk, hd, 1u << (d >> 3));
+    }
+  }
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn g_encode = nullptr;  // set by prompt_configure, before any call
+
+// Rows of [heads][D] as {D, heads, rows}; a box of 64 dimensions, `heads_box` heads, `rows_box`
+// rows lands as lines of 128 bytes with the 128-byte swizzle.  Out-of-range elements read 0.
+bool encode_rows(CUtensorMap *map, const void *ptr, int D, int heads, int64_t rows, int64_t stride, int heads_box,
+                 int rows_box) {
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)stride * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)heads_box, (cuuint32_t)rows_box}, steps[3] = {1, 1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void *>(ptr), dims, strides, box, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int NBOX>
+cudaError_t launch_boxes(const PromptLaunch &L, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm,
+                         bool f16, int ctas, cudaStream_t st) {
+  const bool cap = L.p.softcap != 1.0f;
+  auto go = [&](auto kernel) { kernel<<<ctas, Geo<NBOX>::kThreads, Geo<NBOX>::kSmem, st>>>(L, qm, km, vm); };
+  if (cap && f16) go(prompt_attention_kernel<NBOX, true, true>);
+  else if (cap) go(prompt_attention_kernel<NBOX, true, false>);
+  else if (f16) go(prompt_attention_kernel<NBOX, false, true>);
+  else go(prompt_attention_kernel<NBOX, false, false>);
+  __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -78,16 +692,80 @@ size_t prompt_workspace_bytes(int num_sms, int head_size) {
   const size_t rows = head_size <= 128 ? 256 : 128;
   return (size_t)2 * std::min(num_sms, kMaxPlanCtas) * rows * (head_size + 2) * 4;
 }
-cudaError_t prompt_configure() { return cudaSuccess; }
+
+cudaError_t prompt_configure() {
+  cudaError_t e = cudaSuccess;
+  auto set = [&](auto kernel, int bytes) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  };
+  auto set4 = [&](auto k0, auto k1, auto k2, auto k3, int bytes) {
+    set(k0, bytes), set(k1, bytes), set(k2, bytes), set(k3, bytes);
+  };
+  set4(prompt_attention_kernel<1, false, false>, prompt_attention_kernel<1, false, true>,
+       prompt_attention_kernel<1, true, false>, prompt_attention_kernel<1, true, true>, Geo<1>::kSmem);
+  set4(prompt_attention_kernel<2, false, false>, prompt_attention_kernel<2, false, true>,
+       prompt_attention_kernel<2, true, false>, prompt_attention_kernel<2, true, true>, Geo<2>::kSmem);
+  set4(prompt_attention_kernel<3, false, false>, prompt_attention_kernel<3, false, true>,
+       prompt_attention_kernel<3, true, false>, prompt_attention_kernel<3, true, true>, Geo<3>::kSmem);
+  set4(prompt_attention_kernel<4, false, false>, prompt_attention_kernel<4, false, true>,
+       prompt_attention_kernel<4, true, false>, prompt_attention_kernel<4, true, true>, Geo<4>::kSmem);
+  if (e != cudaSuccess) return e;
+  void *fn = nullptr;
+  cudaDriverEntryPointQueryResult qres;
+  e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres);
+  if (e != cudaSuccess) return e;
+  if (!fn || qres != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+  __atomic_store_n(&g_encode, reinterpret_cast<EncodeFn>(fn), __ATOMIC_RELEASE);
+  return cudaSuccess;
+}
 
 cudaError_t launch_prompt_attention(const PromptParams &p, bool f16, int num_sms, void *workspace, unsigned *err,
                                     cudaStream_t st) {
-  (void)num_sms, (void)workspace, (void)err;
-  const int64_t rows = (int64_t)(p.cu_q[p.S] - p.cu_q[0]) * p.Hq;
-  if (rows <= 0) return cudaSuccess;
-  const unsigned grid = (unsigned)((rows + 3) / 4);
-  if (f16) prompt_rows_kernel<true><<<grid, 128, 0, st>>>(p);
-  else prompt_rows_kernel<false><<<grid, 128, 0, st>>>(p);
+  const PromptShape shape = prompt_shape(p.D, p.G);
+  PromptPlan plan;
+  plan_prompt(p.cu_q, p.cu_kv, 0, p.S, p.Hkv, shape, num_sms, kMinPiece, kMinTilesPerCta, &plan);
+  if (plan.num_ctas == 0) return cudaSuccess;
+  PromptLaunch L;
+  L.p = p;
+  std::copy(plan.begin, plan.begin + plan.num_ctas + 1, L.begin);
+  L.ws = static_cast<float *>(workspace);
+  L.err = err;
+  L.sub_tokens = shape.sub_tokens;
+  L.tile_tokens = shape.tile_tokens;
+  CUtensorMap qm, km, vm;
+  bool ok = encode_rows(&qm, p.q, p.D, p.Hq, p.cu_q[p.S], p.q_stride, p.G, shape.sub_tokens);
+  if (p.cu_kv[p.S] > 0) {
+    ok = ok && encode_rows(&km, p.k, p.D, p.Hkv, p.cu_kv[p.S], p.k_stride, 1, kKeyTile) &&
+         encode_rows(&vm, p.v, p.D, p.Hkv, p.cu_kv[p.S], p.v_stride, 1, kKeyTile);
+  } else {
+    km = vm = qm;  // no key anywhere: never read
+  }
+  if (!ok) return cudaErrorInvalidValue;
+  cudaError_t e = cudaSuccess;
+  switch ((p.D + 63) / 64) {
+    case 1: e = launch_boxes<1>(L, qm, km, vm, f16, plan.num_ctas, st); break;
+    case 2: e = launch_boxes<2>(L, qm, km, vm, f16, plan.num_ctas, st); break;
+    case 3: e = launch_boxes<3>(L, qm, km, vm, f16, plan.num_ctas, st); break;
+    default: e = launch_boxes<4>(L, qm, km, vm, f16, plan.num_ctas, st); break;
+  }
+  if (e != cudaSuccess || plan.num_split == 0) return e;
+  JoinLaunch J;
+  J.p = p;
+  J.ws = L.ws;
+  J.sub_tokens = shape.sub_tokens;
+  J.tile_tokens = shape.tile_tokens;
+  J.rows = shape.tile_tokens > shape.sub_tokens ? 256 : 128;
+  int most = 0;  // rows of the largest item that is cut
+  for (int k = 0; k < plan.num_split; k++) {
+    J.item[k] = plan.begin[plan.split_last[k]];
+    J.first[k] = plan.split_first[k];
+    J.last[k] = plan.split_last[k];
+    const int left = p.cu_q[J.item[k].seq + 1] - p.cu_q[J.item[k].seq] - J.item[k].qt * shape.tile_tokens;
+    most = std::max(most, left > shape.sub_tokens ? J.rows : std::min(left, shape.sub_tokens) * p.G);
+  }
+  const dim3 grid((unsigned)plan.num_split, (unsigned)(most + 31) / 32);
+  if (f16) prompt_join_kernel<true><<<grid, 256, 0, st>>>(J);
+  else prompt_join_kernel<false><<<grid, 256, 0, st>>>(J);
   __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
   return cudaGetLastError();
 }
