@@ -31,7 +31,7 @@ constexpr int kMaxRopePairs = 128;
 // position in units of 2^-64 turns, exact for every 32-bit position up to the entry's own
 // rounding (2^31 * 2^-65 turns): an fp32 or even fp64 product of a far position and a
 // frequency would lose the low bits that the sine depends on.
-struct RopeTable {
+struct alignas(16) RopeTable {
   uint64_t turn[kMaxRopePairs];
   float gain;       // multiplies cosine and sine
   int32_t dims;     // elements rotated, even

@@ -8,14 +8,19 @@
 // position * turn[i] modulo 2^64 in units of 2^-64 turns (RopeTable): reduced exactly, its top
 // 32 bits as a signed number are the angle within half a turn.
 //
-// HBM-bound for chunks, latency-bound for single tokens.  A CTA takes `tokens` tokens (16 for
-// chunks, so that pool stores fill sectors; down to one for small batches, so that the rows
-// spread over the SMs) of one kv head: its key row, its value row and the G query rows.  A row
-// belongs to D / 8 lanes of a warp, 16 bytes each; rows of a group of lanes are loaded four
-// at a time before the first is used.  Sines and cosines are computed once per (token, pair) into
-// shared memory.  The rotation's partner elements sit in the same lane (interleaved pairs), in
+// HBM-bound for chunks, latency-bound for single tokens; in between the instructions count, so
+// that every index is a shift and every address of a loop a constant step.  A CTA takes `tokens`
+// tokens (16 for chunks, so that pool stores fill sectors; down to one for small batches, so that
+// the rows spread over the SMs) of one kv head: its key row, its value row and the G query rows.
+// A row belongs to D / 8 lanes of a warp, 16 bytes each; up to four query rows and the key
+// row of a group of lanes are loaded before the first is used.  A lane computes the sines and cosines of its own elements once
+// per token, in registers.  The rotation's partner elements sit in the same lane (interleaved pairs), in
 // another lane of the group (halves of a multiple of 8 elements: a shuffle) or, for the odd
-// sizes, are read again from global memory.
+// sizes, are read again from global memory.  The value chunk is a transpose of the rows: where a
+// CTA's 16 tokens fill an aligned run of slots it is stored in runs of tokens out of ldmatrix.trans
+// (FP8: byte permutes), otherwise element by element.
+#include <type_traits>
+
 #include "prompt_path.cuh"
 
 namespace pa {
@@ -24,7 +29,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTokMax = 16;
-constexpr int kBatch = 4;  // rows in flight per group of lanes
 enum { PAIR_LANE = 0, PAIR_SHUFFLE = 1, PAIR_MEMORY = 2 };
 
 template <bool F16>
@@ -40,15 +44,24 @@ __device__ __forceinline__ bool has_exponent15(uint2 b) {
   return ((((b.x & 0x78787878u) + 0x08080808u) | ((b.y & 0x78787878u) + 0x08080808u)) & 0x80808080u) != 0u;
 }
 
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
 // GW: lanes of a row, a power of two of at least D / 8.
-template <int GW, bool F16, bool FP8, int PAIR>
-__global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log) {
+// BATCH: query rows in flight per group of lanes: 4, or 1 where a group has no more (less code to
+// fetch on a path whose time is the latency of one pass through it).
+template <int GW, bool F16, bool FP8, int PAIR, int BATCH>
+__global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int G) {
   extern __shared__ __align__(16) uint8_t smem[];
-  const int tokens = 1 << tok_log, D = p.D, half = p.rope.dims >> 1, G = p.Hq / p.Hkv, pieces = D >> 3;
-  const int v_row = D + (FP8 ? 8 : 2);  // elements (FP8: bytes) of a staged value row, padded against bank conflicts
-  float2 *const cs = reinterpret_cast<float2 *>(smem);                   // [tokens][half]
-  uint8_t *const k_s = smem + (size_t)tokens * ((half + 1) & ~1) * 8;    // [tokens][D] elements or bytes
-  uint8_t *const v_s = k_s + (size_t)tokens * D * (FP8 ? 1 : 2);         // [tokens][v_row]
+  const int tokens = 1 << tok_log, D = p.D, dims = p.rope.dims, half = dims >> 1;
+  constexpr int kElem = FP8 ? 1 : 2;  // bytes of a pool element
+  const int v_row = D * kElem + 16;   // bytes of a staged value row, padded against bank conflicts
+  uint8_t *const k_s = smem;                                             // [tokens][D]
+  uint8_t *const v_s = k_s + tokens * D * kElem;                         // [tokens][v_row]
   __shared__ int64_t slot_s[kTokMax];
 
   // the attention kernel that follows may set up (it reads no pool data before its own wait)
@@ -58,195 +71,267 @@ __global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __gr
   const int n_tok = (int)min((int64_t)tokens, p.num_tokens - t0);
   const bool write = p.slot_mapping != nullptr;
 
-  // ---- this group's rows: token, then every `share`-th of (key, G queries) -------------
+  // ---- this group's rows: of one token, every `share`-th query row; the last group has the key --
   constexpr int kGroups = kThreads / GW;
   const int group = tid / GW, gl = tid % GW, e0 = gl * 8;
-  const int share = kGroups >= tokens ? kGroups >> tok_log : 1;  // groups of a token
+  const uint32_t lanes = (GW == 32 ? 0xffffffffu : (1u << (GW % 32)) - 1u) << ((tid & 31) / GW * GW);  // this group's
   const bool in_row = e0 < D;
-  auto row_src = [&](int64_t t, int r) {
-    return r == 0 ? p.k + t * p.k_stride + (int64_t)h * D : p.q + t * p.q_stride + (int64_t)(h * G + r - 1) * D;
-  };
-  uint4 raw[kBatch];
-  auto load_batch = [&](int tok, int r0) {
+  const int share_log = kGroups >> tok_log ? 31 - __clz(kGroups >> tok_log) : 0;  // log2(groups of a token)
+  const int share = 1 << share_log, first = group & (share - 1);
+  int tok = group >> share_log;
+  const elem16 *q_src;  // this lane's piece of the token's first query row
+  uint4 raw[BATCH], raw_k;
+  auto load_q = [&](int r0) {
 #pragma unroll
-    for (int b = 0; b < kBatch; b++) {
-      const int r = r0 + b * share;
+    for (int b = 0; b < BATCH; b++) {
+      const int r = r0 + (b << share_log);
       raw[b] = make_uint4(0, 0, 0, 0);
-      if (in_row && tok < n_tok && r <= G) raw[b] = *reinterpret_cast<const uint4 *>(row_src(t0 + tok, r) + e0);
+      if (in_row && tok < n_tok && r < G) raw[b] = *reinterpret_cast<const uint4 *>(q_src + r * D);
     }
   };
-  int tok = group / share;
-  const int r_first = group % share;
-  load_batch(tok, r_first);
-  uint4 qw = make_uint4(0, 0, 0, 0), kw = qw;
-  if (in_row && p.q_norm_w) qw = *reinterpret_cast<const uint4 *>(p.q_norm_w + e0);
-  if (in_row && p.k_norm_w) kw = *reinterpret_cast<const uint4 *>(p.k_norm_w + e0);
+  auto load_token = [&] {
+    q_src = p.q + (t0 + tok) * p.q_stride + (int64_t)h * G * D + e0;
+    raw_k = make_uint4(0, 0, 0, 0);
+    if (in_row && tok < n_tok && first == share - 1)
+      raw_k = *reinterpret_cast<const uint4 *>(p.k + (t0 + tok) * p.k_stride + h * D + e0);
+    load_q(first);
+  };
+  load_token();
+  const bool turns = e0 < dims;  // this lane has elements that rotate (PAIR_SHUFFLE: all of them or none)
+  // the piece with the partners of this lane's elements (PAIR_SHUFFLE), in lanes
+  const int other = PAIR != PAIR_SHUFFLE || !turns ? gl : e0 < half ? gl + (half >> 3) : gl - (half >> 3);
+  auto partner = [&](int d) { return PAIR == PAIR_LANE ? d ^ 1 : d < half ? d + half : d - half; };
 
-  // ---- slots, values, sines -------------------------------------------------------------
-  if (tid < kTokMax) {
-    int64_t s = -1;
-    if (write && tid < n_tok) {
-      s = p.slot_mapping[t0 + tid];
-      if (s >= ((int64_t)p.num_blocks << p.bs_log)) {
-        atomicOr(p.err, kErrSlotRange);
-        s = -1;
-      }
+  // The plan's entries of this lane's elements (of its four pairs, when they are interleaved).  An
+  // indexed constant load takes a cycle and more per distinct address of a warp; through a generic
+  // address it is an ordinary load.
+  constexpr int kTurns = PAIR == PAIR_LANE ? 4 : 8;
+  uint32_t turn_lo[kTurns], turn_hi[kTurns];
+  if (PAIR == PAIR_MEMORY) {
+#pragma unroll
+    for (int i = 0; i < kTurns; i++) {
+      const int d = e0 + i;
+      turn_lo[i] = turn_hi[i] = 0;
+      if (d < dims)
+        asm("ld.v2.u32 {%0, %1}, [%2];" : "=r"(turn_lo[i]), "=r"(turn_hi[i]) : "l"(p.rope.turn + (d < half ? d : d - half)));
     }
-    slot_s[tid] = s;
+  } else {
+    const uint64_t *at = p.rope.turn + (!turns ? 0 : PAIR == PAIR_LANE ? e0 >> 1 : e0 < half ? e0 : e0 - half);
+#pragma unroll
+    for (int i = 0; i < kTurns; i += 2)
+      asm("ld.v4.u32 {%0, %1, %2, %3}, [%4];"
+          : "=r"(turn_lo[i]), "=r"(turn_hi[i]), "=r"(turn_lo[i + 1]), "=r"(turn_hi[i + 1])
+          : "l"(at + i));
   }
+
+  // ---- slots and values ---------------------------------------------------------------------
   if (write) {
-    for (int i = tid; i < n_tok * pieces; i += kThreads) {
-      const int vt = i / pieces, c = i - vt * pieces;
-      const uint4 v = *reinterpret_cast<const uint4 *>(p.v + (t0 + vt) * p.v_stride + (int64_t)h * D + c * 8);
+    if (tid < tokens) {
+      int64_t s = -1;
+      if (tid < n_tok) {
+        s = p.slot_mapping[t0 + tid];
+        if (s >= ((int64_t)p.num_blocks << p.bs_log)) {
+          atomicOr(p.err, kErrSlotRange);
+          s = -1;
+        }
+      }
+      slot_s[tid] = s;
+    }
+    for (int vt = group; vt < n_tok; vt += kGroups) {
+      if (!in_row) break;
+      const uint4 v = *reinterpret_cast<const uint4 *>(p.v + (t0 + vt) * p.v_stride + h * D + e0);
       if (FP8) {
         const uint2 b = quantise8<F16>(v, p.v_scale);
         if (has_exponent15(b) && p.slot_mapping[t0 + vt] >= 0) atomicOr(p.special, 1u);
-        *reinterpret_cast<uint2 *>(v_s + vt * v_row + c * 8) = b;
+        *reinterpret_cast<uint2 *>(v_s + vt * v_row + e0) = b;
       } else {
-        uint32_t *d = reinterpret_cast<uint32_t *>(v_s + (vt * v_row + c * 8) * 2);
-        d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+        *reinterpret_cast<uint4 *>(v_s + vt * v_row + e0 * 2) = v;
       }
     }
   }
-  for (int i = tid; i < n_tok * half; i += kThreads) {
-    const int ct = i / half, f = i - ct * half;
-    const uint64_t phase = (uint64_t)(int64_t)p.positions[t0 + ct] * p.rope.turn[f];
-    float sn, cn;
-    sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &sn, &cn);
-    cs[ct * half + f] = make_float2(cn * p.rope.gain, sn * p.rope.gain);
-  }
-  __syncthreads();
 
-  // ---- norm and rotation --------------------------------------------------------------------
-  const int step = kGroups >= tokens ? tokens : kGroups;  // a group takes tokens `step` apart
-  for (; tok < tokens; tok += step) {
-    if (tok != group / share) load_batch(tok, r_first);
-    // sine and cosine of this lane's elements (of its four pairs, when they are interleaved)
-    float co[8], si[8];
+  // ---- norm and rotation: y_e = inv (x_e A_e + x_partner B_e) ------------------------------------
+  const float inv_d = 1.f / (float)D;
+  // A *= w, B *= the partner's w
+  auto weigh = [&](const elem16 *w, float (&A)[8], float (&B)[8]) {
+    float wv[8];
+    unpack8<F16>(*reinterpret_cast<const uint4 *>(w + e0), wv);
+#pragma unroll
+    for (int i = 0; i < 8; i++) A[i] *= wv[i];
+    if (PAIR == PAIR_LANE) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) B[i] *= wv[i ^ 1];
+    } else if (PAIR == PAIR_SHUFFLE) {
+      unpack8<F16>(*reinterpret_cast<const uint4 *>(w + other * 8), wv);
+#pragma unroll
+      for (int i = 0; i < 8; i++) B[i] *= wv[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+        if (e0 + i < dims) B[i] *= elem_value<F16>(w[partner(e0 + i)]);
+    }
+  };
+  // one row of this group: its piece in `r`, its address (PAIR_MEMORY) in `src`
+  auto turn_row = [&](uint4 r, const elem16 *src, bool norm, const float (&A)[8], const float (&B)[8]) {
+    float x[8], z[8];
+    unpack8<F16>(r, x);
+    float inv = 1.f;
+    if (norm) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+      for (int o = GW / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
+      inv = rsqrtf(fmaf(ss, inv_d, p.eps));
+    }
+    // the partner's value, 0 for an element that does not rotate (its B is 0, and 0 * inf is not)
+    if (PAIR == PAIR_LANE) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) z[i] = e0 + i < dims ? x[i ^ 1] : 0.f;
+    } else if (PAIR == PAIR_SHUFFLE) {
+      uint4 o;
+      o.x = __shfl_sync(lanes, r.x, other, GW);
+      o.y = __shfl_sync(lanes, r.y, other, GW);
+      o.z = __shfl_sync(lanes, r.z, other, GW);
+      o.w = __shfl_sync(lanes, r.w, other, GW);
+      if (!turns) o = make_uint4(0, 0, 0, 0);
+      unpack8<F16>(o, z);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) z[i] = in_row && e0 + i < dims ? elem_value<F16>(src[partner(e0 + i) - e0]) : 0.f;
+      __syncwarp(lanes);  // the row may be rotated in place: all of it has been read
+    }
+    uint32_t out[4];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+      out[i >> 1] = pack2<F16>(fmaf(x[i], A[i], z[i] * B[i]) * inv, fmaf(x[i + 1], A[i + 1], z[i + 1] * B[i + 1]) * inv);
+    return make_uint4(out[0], out[1], out[2], out[3]);
+  };
+  for (;;) {
     if (tok < n_tok) {
+      // Sine and cosine for this lane's elements.  The phase's top word is within half a turn, where
+      // the hardware's sine and cosine are off by at most 2^-20.9 absolute: nothing against the
+      // half step of 2^-9 or 2^-12 that the result is rounded by.
+      const int64_t t = t0 + tok;
+      const int32_t pos = p.positions[t];
+      float A[8], B[8];
 #pragma unroll
-      for (int i = 0; i < (PAIR == PAIR_LANE ? 4 : 8); i++) {
-        const int d = PAIR == PAIR_LANE ? e0 + 2 * i : e0 + i;
-        float2 c = make_float2(1.f, 0.f);
-        if (d < 2 * half) c = cs[tok * half + (PAIR == PAIR_LANE ? d >> 1 : d < half ? d : d - half)];
-        co[i] = c.x;
-        si[i] = PAIR == PAIR_LANE || d >= half ? c.y : -c.y;  // halves: first a cos - b sin, second b cos + a sin
-      }
-    }
-    const int64_t t = t0 + tok;
-    // the same number of rounds for every group of a warp: they meet at the shuffles
-    for (int r0 = r_first; r0 - r_first <= G; r0 += kBatch * share) {
-      if (r0 != r_first) load_batch(tok, r0);
-#pragma unroll
-      for (int b = 0; b < kBatch; b++) {
-        const int r = r0 + b * share;
-        // (shuffles below: groups of one warp may hold different rows, or none)
-        const bool have = in_row && tok < n_tok && r <= G;
-        const bool is_k = r == 0, norm = is_k ? p.k_norm_w != nullptr : p.q_norm_w != nullptr;
-        float x[8], y[8];
-        unpack8<F16>(raw[b], x);
-        float inv = 1.f;
-        if (p.q_norm_w || p.k_norm_w) {
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-          for (int o = GW / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          if (norm) {
-            inv = rsqrtf(ss / (float)D + p.eps);
-            float w[8];
-            unpack8<F16>(is_k ? kw : qw, w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= inv * w[i];
-          }
-        }
+      for (int i = 0; i < kTurns; i++) {
+        // top word of (64-bit position) * entry modulo 2^64
+        uint32_t phase = __umulhi((uint32_t)pos, turn_lo[i]) + (uint32_t)pos * turn_hi[i];
+        phase -= (uint32_t)(pos >> 31) & turn_lo[i];
+        const float angle = (float)(int32_t)phase * 1.46291807926715968e-9f;  // 2 pi / 2^32
+        const float cn = __cosf(angle) * p.rope.gain, sn = __sinf(angle) * p.rope.gain;
         if (PAIR == PAIR_LANE) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            y[2 * i] = x[2 * i] * co[i] - x[2 * i + 1] * si[i];
-            y[2 * i + 1] = x[2 * i + 1] * co[i] + x[2 * i] * si[i];
-          }
-        } else if (PAIR == PAIR_SHUFFLE) {
-          const int other = e0 < half ? gl + (half >> 3) : gl - (half >> 3);  // used below 2 * half only
-          const bool turns = e0 < 2 * half;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const float z = __shfl_sync(0xffffffffu, x[i], turns ? other : gl, GW);
-            y[i] = turns ? fmaf(x[i], co[i], z * si[i]) : x[i];
-          }
+          const bool on = e0 + 2 * i < dims;
+          A[2 * i] = A[2 * i + 1] = on ? cn : 1.f;
+          B[2 * i] = on ? -sn : 0.f;
+          B[2 * i + 1] = on ? sn : 0.f;
         } else {
-          const elem16 *src = row_src(t, r), *w = is_k ? p.k_norm_w : p.q_norm_w;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            const int d = e0 + i;
-            y[i] = x[i];
-            if (have && d < 2 * half) {
-              const int o = d < half ? d + half : d - half;
-              float z = elem_value<F16>(src[o]);
-              if (norm) z *= inv * elem_value<F16>(w[o]);
-              y[i] = fmaf(x[i], co[i], z * si[i]);
-            }
-          }
-          __syncwarp();  // the row may be rotated in place: all of it has been read
+          const bool on = e0 + i < dims;
+          A[i] = on ? cn : 1.f;
+          B[i] = on ? (e0 + i < half ? -sn : sn) : 0.f;
         }
-        if (have) {
-          const uint4 out = make_uint4(pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3]), pack2<F16>(y[4], y[5]), pack2<F16>(y[6], y[7]));
-          if (!is_k) {
-            *reinterpret_cast<uint4 *>(p.q_out + t * p.q_out_stride + (int64_t)(h * G + r - 1) * D + e0) = out;
-          } else {
-            if (p.k_out) *reinterpret_cast<uint4 *>(p.k_out + t * p.k_out_stride + (int64_t)h * D + e0) = out;
-            if (write && FP8) {
-              const uint2 q8 = quantise8<F16>(out, p.k_scale);
-              if (has_exponent15(q8) && slot_s[tok] >= 0) atomicOr(p.special, 1u);
-              *reinterpret_cast<uint2 *>(k_s + tok * D + e0) = q8;
-            } else if (write) {
-              *reinterpret_cast<uint4 *>(k_s + (tok * D + e0) * 2) = out;
-            }
+      }
+      if (first == share - 1) {  // the key row
+        float Ak[8], Bk[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) Ak[i] = A[i], Bk[i] = B[i];
+        if (p.k_norm_w && in_row) weigh(p.k_norm_w, Ak, Bk);
+        const uint4 out = turn_row(raw_k, p.k + t * p.k_stride + h * D + e0, p.k_norm_w != nullptr, Ak, Bk);
+        if (in_row) {
+          if (p.k_out) *reinterpret_cast<uint4 *>(p.k_out + t * p.k_out_stride + h * D + e0) = out;
+          if (write && FP8) {
+            const uint2 q8 = quantise8<F16>(out, p.k_scale);
+            if (has_exponent15(q8) && p.slot_mapping[t] >= 0) atomicOr(p.special, 1u);
+            *reinterpret_cast<uint2 *>(k_s + tok * D + e0) = q8;
+          } else if (write) {
+            *reinterpret_cast<uint4 *>(k_s + (tok * D + e0) * 2) = out;
           }
         }
       }
+      if (p.q_norm_w && in_row) weigh(p.q_norm_w, A, B);
+      elem16 *const q_dst = p.q_out + t * p.q_out_stride + (int64_t)h * G * D + e0;
+      for (int base = first; base < G; base += BATCH << share_log) {
+        if (base != first) load_q(base);
+#pragma unroll
+        for (int b = 0; b < BATCH; b++) {
+          const int r = base + (b << share_log);
+          if (r >= G) break;
+          const uint4 out = turn_row(raw[b], q_src + r * D, p.q_norm_w != nullptr, A, B);
+          if (in_row) *reinterpret_cast<uint4 *>(q_dst + r * D) = out;
+        }
+      }
     }
+    // fewer groups than tokens (rows of 32 lanes): a group takes a second token
+    tok += kGroups;
+    if (tok >= tokens) break;
+    load_token();
   }
   if (!write) return;
   __syncthreads();
 
-  // ---- pool write, token index fastest across threads ---------------------------------------
-  const int bs = 1 << p.bs_log;
-  constexpr int X = FP8 ? 16 : 8;  // elements of a 16-byte key piece
-  for (int i = tid; i < (D / X) << tok_log; i += kThreads) {
-    const int wt = i & (tokens - 1), c = i >> tok_log;
-    const int64_t slot = slot_s[wt];
-    if (slot < 0) continue;
-    const int64_t chunk = ((slot >> p.bs_log) * p.Hkv + h) * (int64_t)D << p.bs_log;
-    const int off = (int)(slot & (bs - 1));
-    uint8_t *dst = static_cast<uint8_t *>(p.k_pool) + (chunk + (int64_t)(c * bs + off) * X) * (FP8 ? 1 : 2);
-    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(k_s + wt * D * (FP8 ? 1 : 2) + c * 16);
+  // ---- pool write, token index fastest across threads: a thread keeps its token ----------------
+  const int wt = tid & (tokens - 1), bs = 1 << p.bs_log;
+  const int64_t slot = slot_s[wt];
+  const int off = (int)(slot & (bs - 1));
+  const int64_t chunk = (((slot >> p.bs_log) * p.Hkv + h) * (int64_t)D << p.bs_log) * kElem;  // bytes
+  if (slot >= 0) {
+    uint8_t *dst = static_cast<uint8_t *>(p.k_pool) + chunk + off * 16;
+    for (int c = tid >> tok_log; c < D * kElem / 16; c += kThreads >> tok_log)
+      *reinterpret_cast<uint4 *>(dst + c * bs * 16) = *reinterpret_cast<const uint4 *>(k_s + wt * D * kElem + c * 16);
   }
-  for (int i = tid; i < D << tok_log; i += kThreads) {
-    const int wt = i & (tokens - 1), d = i >> tok_log;
-    const int64_t slot = slot_s[wt];
-    if (slot < 0) continue;
-    const int64_t at = (((slot >> p.bs_log) * p.Hkv + h) * (int64_t)D << p.bs_log) + (int64_t)d * bs + (slot & (bs - 1));
-    if (FP8) static_cast<uint8_t *>(p.v_pool)[at] = v_s[wt * v_row + d];
-    else static_cast<elem16 *>(p.v_pool)[at] = *reinterpret_cast<const elem16 *>(v_s + (wt * v_row + d) * 2);
+  // an aligned run of 16 slots (two blocks of 8 tokens are not one)
+  const bool run = __all_sync(0xffffffffu, tokens == kTokMax && bs >= kTokMax && slot >= 0 && slot == slot_s[0] + wt && (slot_s[0] & 15) == 0);
+  const int warp = tid >> 5, lane = tid & 31;
+  if (run && !FP8) {
+    // matrices 0 and 1 hold 8 dimensions, 2 and 3 the next 8; row r of matrix m is token
+    // (r / 2) * 4 + 2 (m % 2) + r % 2, so that a lane ends up with four tokens of a dimension
+    const int m = lane >> 3, r = lane & 7, mt = (r >> 1) * 4 + (m & 1) * 2 + (r & 1);
+    const int64_t run_at = chunk + (slot_s[0] & (bs - 1)) * 2;
+    for (int d0 = warp * 16; d0 < D; d0 += kThreads / 2) {
+      uint32_t w[4];
+      ldmatrix_x4_trans(w, smem_u32(v_s) + mt * v_row + (d0 + (m >> 1) * 8) * 2);
+      uint8_t *dst = static_cast<uint8_t *>(p.v_pool) + run_at + (lane & 3) * 8;
+      const int d = d0 + (lane >> 2);
+      *reinterpret_cast<uint2 *>(dst + (int64_t)d * bs * 2) = make_uint2(w[0], w[1]);
+      if (d + 8 < D) *reinterpret_cast<uint2 *>(dst + (int64_t)(d + 8) * bs * 2) = make_uint2(w[2], w[3]);
+    }
+  } else if (run) {
+    // four tokens x four dimensions of bytes per thread
+    if (tid < D) {
+      const int tq = tid & 3, d = (tid >> 2) * 4;
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint32_t *>(v_s + (tq * 4 + i) * v_row + d);
+      const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);  // dimensions 0, 1
+      const uint32_t c = __byte_perm(w[0], w[1], 0x7362), e = __byte_perm(w[2], w[3], 0x7362);  // dimensions 2, 3
+      uint8_t *dst = static_cast<uint8_t *>(p.v_pool) + chunk + (slot_s[0] & (bs - 1)) + tq * 4 + d * bs;
+      *reinterpret_cast<uint32_t *>(dst) = __byte_perm(a, b, 0x5410);
+      *reinterpret_cast<uint32_t *>(dst + bs) = __byte_perm(a, b, 0x7632);
+      *reinterpret_cast<uint32_t *>(dst + 2 * bs) = __byte_perm(c, e, 0x5410);
+      *reinterpret_cast<uint32_t *>(dst + 3 * bs) = __byte_perm(c, e, 0x7632);
+    }
+  } else if (slot >= 0) {
+    for (int d = tid >> tok_log; d < D; d += kThreads >> tok_log) {
+      if (FP8) static_cast<uint8_t *>(p.v_pool)[chunk + d * bs + off] = v_s[wt * v_row + d];
+      else static_cast<elem16 *>(p.v_pool)[chunk / 2 + d * bs + off] = *reinterpret_cast<const elem16 *>(v_s + wt * v_row + d * 2);
+    }
   }
 }
 
-template <int GW, bool FP8>
-cudaError_t launch_group(const RotateParams &p, bool f16, int tok_log, dim3 grid, size_t smem, cudaStream_t st) {
-  const int half = p.rope.dims / 2;
-  auto go = [&](auto kernel) { kernel<<<grid, kThreads, smem, st>>>(p, tok_log); };
-  if (p.rope.interleaved) {
-    if (f16) go(rope_norm_cache_kernel<GW, true, FP8, PAIR_LANE>);
-    else go(rope_norm_cache_kernel<GW, false, FP8, PAIR_LANE>);
-  } else if (half % 8 == 0) {
-    if (f16) go(rope_norm_cache_kernel<GW, true, FP8, PAIR_SHUFFLE>);
-    else go(rope_norm_cache_kernel<GW, false, FP8, PAIR_SHUFFLE>);
-  } else {
-    if (f16) go(rope_norm_cache_kernel<GW, true, FP8, PAIR_MEMORY>);
-    else go(rope_norm_cache_kernel<GW, false, FP8, PAIR_MEMORY>);
-  }
+template <int GW, bool FP8, bool F16, int PAIR>
+cudaError_t launch_pair(const RotateParams &p, int tok_log, dim3 grid, size_t smem, cudaStream_t st) {
+  const int G = p.Hq / p.Hkv, share = (kThreads / GW) >> tok_log;  // groups of a token
+  if (share >= G) rope_norm_cache_kernel<GW, F16, FP8, PAIR, 1><<<grid, kThreads, smem, st>>>(p, tok_log, G);
+  else rope_norm_cache_kernel<GW, F16, FP8, PAIR, 4><<<grid, kThreads, smem, st>>>(p, tok_log, G);
   return cudaGetLastError();
+}
+template <int GW, bool FP8, bool F16>
+cudaError_t launch_group(const RotateParams &p, int tok_log, dim3 grid, size_t smem, cudaStream_t st) {
+  if (p.rope.interleaved) return launch_pair<GW, FP8, F16, PAIR_LANE>(p, tok_log, grid, smem, st);
+  if (p.rope.dims % 16 == 0) return launch_pair<GW, FP8, F16, PAIR_SHUFFLE>(p, tok_log, grid, smem, st);
+  return launch_pair<GW, FP8, F16, PAIR_MEMORY>(p, tok_log, grid, smem, st);
 }
 
 }  // namespace
@@ -256,15 +341,18 @@ cudaError_t launch_rope_norm_cache(const RotateParams &p, bool f16, bool fp8, in
   // about two CTAs per SM before a CTA takes more than one token
   int tok_log = 0;
   while (tok_log < 4 && (p.num_tokens * p.Hkv >> (tok_log + 1)) >= 2 * num_sms) tok_log++;
-  const int tokens = 1 << tok_log, half = p.rope.dims / 2;
+  const int tokens = 1 << tok_log;
   const dim3 grid((unsigned)((p.num_tokens + tokens - 1) >> tok_log), (unsigned)p.Hkv);
-  const size_t smem = (size_t)tokens * (((half + 1) & ~1) * 8 + (fp8 ? 2 * p.D + 8 : 4 * p.D + 4));
-  cudaError_t e;
-  if (fp8) e = launch_group<16, true>(p, f16, tok_log, grid, smem, st);
-  else if (p.D <= 32) e = launch_group<4, false>(p, f16, tok_log, grid, smem, st);
-  else if (p.D <= 64) e = launch_group<8, false>(p, f16, tok_log, grid, smem, st);
-  else if (p.D <= 128) e = launch_group<16, false>(p, f16, tok_log, grid, smem, st);
-  else e = launch_group<32, false>(p, f16, tok_log, grid, smem, st);
+  const size_t smem = (size_t)tokens * (p.D * (fp8 ? 2 : 4) + 16);
+  auto go = [&](auto f16_tag) {
+    constexpr bool F16 = decltype(f16_tag)::value;
+    if (fp8) return launch_group<16, true, F16>(p, tok_log, grid, smem, st);
+    if (p.D <= 32) return launch_group<4, false, F16>(p, tok_log, grid, smem, st);
+    if (p.D <= 64) return launch_group<8, false, F16>(p, tok_log, grid, smem, st);
+    if (p.D <= 128) return launch_group<16, false, F16>(p, tok_log, grid, smem, st);
+    return launch_group<32, false, F16>(p, tok_log, grid, smem, st);
+  };
+  const cudaError_t e = f16 ? go(std::true_type{}) : go(std::false_type{});
   __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
   return e;
 }
