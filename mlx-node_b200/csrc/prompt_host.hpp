@@ -123,7 +123,7 @@ inline ArgError check_rotate_args(const PagedAttnConfig &cfg, const RopeTable *r
   if (!slot_mapping && !k_out) return bad_arg("slot_mapping and k_out are both null: the keys would go nowhere");
   if (slot_mapping && !v) return bad_arg("v is null");
   if (num_q_heads <= 0 || num_q_heads % Hkv) return bad_arg("num_q_heads must be a positive multiple of num_kv_heads");
-  if (Hkv > 65535) return bad_arg("more than 65535 kv heads");
+  if (Hkv + num_q_heads > 65535) return bad_arg("more than 65535 heads");
   if (!(eps >= 0.f) || !std::isfinite(eps)) return bad_arg("eps must be finite and >= 0");
   const int64_t q_row = num_q_heads * D, kv_row = Hkv * D;
   if (q_stride < q_row || q_out_stride < q_row || k_stride < kv_row || (k_out && k_out_stride < kv_row) ||

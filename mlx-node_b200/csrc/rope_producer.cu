@@ -9,16 +9,22 @@
 // 32 bits as a signed number are the angle within half a turn.
 //
 // HBM-bound for chunks, latency-bound for single tokens; in between the instructions count, so
-// that every index is a shift and every address of a loop a constant step.  A CTA takes `tokens`
-// tokens (16 for chunks, so that pool stores fill sectors; down to one for small batches, so that
-// the rows spread over the SMs) of one kv head: its key row, its value row and the G query rows.
-// A row belongs to D / 8 lanes of a warp, 16 bytes each; up to four query rows and the key
-// row of a group of lanes are loaded before the first is used.  A lane computes the sines and cosines of its own elements once
-// per token, in registers.  The rotation's partner elements sit in the same lane (interleaved pairs), in
-// another lane of the group (halves of a multiple of 8 elements: a shuffle) or, for the odd
-// sizes, are read again from global memory.  The value chunk is a transpose of the rows: where a
-// CTA's 16 tokens fill an aligned run of slots it is stored in runs of tokens out of ldmatrix.trans
-// (FP8: byte permutes), otherwise element by element.
+// that every index is a shift and every address of a loop a constant step.  Two kinds of CTAs, both
+// over `tokens` tokens - 16 for chunks, so that pool stores fill sectors; down to one for small
+// batches, so that the rows spread over the SMs:
+//   queries    up to 16 query heads of the tokens; nothing is shared, no barrier
+//   keys       up to 4 kv heads: the key rows, the value rows and the pool write, staged in shared
+//              memory
+// (more heads to a CTA where it has few tokens: what a CTA does once - addresses, the plan's entries,
+// sines - costs as much as three rows).
+// A row belongs to D / 8 lanes of a warp, 16 bytes each; up to four query rows of a group of lanes
+// are loaded before the first is used.  A lane computes the sines and cosines of its own elements
+// once per token, in registers, and folds the norm's weights into them.  The rotation's partner
+// elements sit in the same lane (interleaved pairs), in another lane of the group (halves of a
+// multiple of 8 elements: a shuffle) or, for the odd sizes, are read again from global memory.  The
+// value chunk is a transpose of the rows: where a CTA's 16 tokens fill an aligned run of slots it is
+// stored in runs of tokens out of ldmatrix.trans (FP8: byte permutes), otherwise element by element.
+#include <algorithm>
 #include <type_traits>
 
 #include "prompt_path.cuh"
@@ -55,48 +61,49 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 // BATCH: query rows in flight per group of lanes: 4, or 1 where a group has no more (less code to
 // fetch on a path whose time is the latency of one pass through it).
 template <int GW, bool F16, bool FP8, int PAIR, int BATCH>
-__global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int G) {
+__global__ void __launch_bounds__(kThreads, BATCH == 1 ? 3 : 4)
+rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int q_heads, int kv_heads, int kv_ctas) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int tokens = 1 << tok_log, D = p.D, dims = p.rope.dims, half = dims >> 1;
   constexpr int kElem = FP8 ? 1 : 2;  // bytes of a pool element
   const int v_row = D * kElem + 16;   // bytes of a staged value row, padded against bank conflicts
-  uint8_t *const k_s = smem;                                             // [tokens][D]
-  uint8_t *const v_s = k_s + tokens * D * kElem;                         // [tokens][v_row]
   __shared__ int64_t slot_s[kTokMax];
 
   // the attention kernel that follows may set up (it reads no pool data before its own wait)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int h = blockIdx.y, tid = threadIdx.x;
+  const int tid = threadIdx.x;
+  const bool keys = (int)blockIdx.y < kv_ctas;
+  const int h = keys ? blockIdx.y * kv_heads : (blockIdx.y - kv_ctas) * q_heads;  // first head
+  const int n_heads = keys ? min(kv_heads, p.Hkv - h) : min(q_heads, p.Hq - h);   // rows of a token
+  uint8_t *const k_s = smem;                                  // [head][token][D]
+  uint8_t *const v_s = k_s + kv_heads * tokens * D * kElem;   // [head][token][v_row]
   const int64_t t0 = (int64_t)blockIdx.x << tok_log;
   const int n_tok = (int)min((int64_t)tokens, p.num_tokens - t0);
-  const bool write = p.slot_mapping != nullptr;
+  const bool write = keys && p.slot_mapping != nullptr;
 
-  // ---- this group's rows: of one token, every `share`-th query row; the last group has the key --
+  // ---- this group's rows: of one token, every `share`-th row ------------------------------
   constexpr int kGroups = kThreads / GW;
   const int group = tid / GW, gl = tid % GW, e0 = gl * 8;
   const uint32_t lanes = (GW == 32 ? 0xffffffffu : (1u << (GW % 32)) - 1u) << ((tid & 31) / GW * GW);  // this group's
   const bool in_row = e0 < D;
   const int share_log = kGroups >> tok_log ? 31 - __clz(kGroups >> tok_log) : 0;  // log2(groups of a token)
-  const int share = 1 << share_log, first = group & (share - 1);
+  const int first = group & ((1 << share_log) - 1);
   int tok = group >> share_log;
-  const elem16 *q_src;  // this lane's piece of the token's first query row
-  uint4 raw[BATCH], raw_k;
-  auto load_q = [&](int r0) {
+  const elem16 *const x_in = (keys ? p.k : p.q) + (t0 * (keys ? p.k_stride : p.q_stride) + (int64_t)h * D + e0);
+  const int64_t x_stride = keys ? p.k_stride : p.q_stride;
+  const elem16 *const weight = keys ? p.k_norm_w : p.q_norm_w;
+  const elem16 *src;  // this lane's piece of the token's first row
+  uint4 raw[BATCH];
+  auto load_rows = [&](int r0) {
 #pragma unroll
     for (int b = 0; b < BATCH; b++) {
       const int r = r0 + (b << share_log);
       raw[b] = make_uint4(0, 0, 0, 0);
-      if (in_row && tok < n_tok && r < G) raw[b] = *reinterpret_cast<const uint4 *>(q_src + r * D);
+      if (in_row && tok < n_tok && r < n_heads) raw[b] = *reinterpret_cast<const uint4 *>(src + r * D);
     }
   };
-  auto load_token = [&] {
-    q_src = p.q + (t0 + tok) * p.q_stride + (int64_t)h * G * D + e0;
-    raw_k = make_uint4(0, 0, 0, 0);
-    if (in_row && tok < n_tok && first == share - 1)
-      raw_k = *reinterpret_cast<const uint4 *>(p.k + (t0 + tok) * p.k_stride + h * D + e0);
-    load_q(first);
-  };
-  load_token();
+  src = x_in + tok * x_stride;
+  load_rows(first);
   const bool turns = e0 < dims;  // this lane has elements that rotate (PAIR_SHUFFLE: all of them or none)
   // the piece with the partners of this lane's elements (PAIR_SHUFFLE), in lanes
   const int other = PAIR != PAIR_SHUFFLE || !turns ? gl : e0 < half ? gl + (half >> 3) : gl - (half >> 3);
@@ -137,46 +144,29 @@ __global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __gr
       }
       slot_s[tid] = s;
     }
-    for (int vt = group; vt < n_tok; vt += kGroups) {
-      if (!in_row) break;
-      const uint4 v = *reinterpret_cast<const uint4 *>(p.v + (t0 + vt) * p.v_stride + h * D + e0);
-      if (FP8) {
-        const uint2 b = quantise8<F16>(v, p.v_scale);
-        if (has_exponent15(b) && p.slot_mapping[t0 + vt] >= 0) atomicOr(p.special, 1u);
-        *reinterpret_cast<uint2 *>(v_s + vt * v_row + e0) = b;
-      } else {
-        *reinterpret_cast<uint4 *>(v_s + vt * v_row + e0 * 2) = v;
+    for (int vt = tok; vt < n_tok; vt += kGroups) {
+      for (int r = first; r < n_heads && in_row; r += 1 << share_log) {
+        const elem16 *v = p.v + (t0 + vt) * p.v_stride + (h + r) * D + e0;
+        uint8_t *dst = v_s + (r * tokens + vt) * v_row + e0 * kElem;
+        if (FP8) {
+          const uint2 b = quantise8<F16>(*reinterpret_cast<const uint4 *>(v), p.v_scale);
+          if (has_exponent15(b) && p.slot_mapping[t0 + vt] >= 0) atomicOr(p.special, 1u);
+          *reinterpret_cast<uint2 *>(dst) = b;
+        } else {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(v) : "memory");
+        }
       }
     }
   }
 
   // ---- norm and rotation: y_e = inv (x_e A_e + x_partner B_e) ------------------------------------
   const float inv_d = 1.f / (float)D;
-  // A *= w, B *= the partner's w
-  auto weigh = [&](const elem16 *w, float (&A)[8], float (&B)[8]) {
-    float wv[8];
-    unpack8<F16>(*reinterpret_cast<const uint4 *>(w + e0), wv);
-#pragma unroll
-    for (int i = 0; i < 8; i++) A[i] *= wv[i];
-    if (PAIR == PAIR_LANE) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) B[i] *= wv[i ^ 1];
-    } else if (PAIR == PAIR_SHUFFLE) {
-      unpack8<F16>(*reinterpret_cast<const uint4 *>(w + other * 8), wv);
-#pragma unroll
-      for (int i = 0; i < 8; i++) B[i] *= wv[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i++)
-        if (e0 + i < dims) B[i] *= elem_value<F16>(w[partner(e0 + i)]);
-    }
-  };
-  // one row of this group: its piece in `r`, its address (PAIR_MEMORY) in `src`
-  auto turn_row = [&](uint4 r, const elem16 *src, bool norm, const float (&A)[8], const float (&B)[8]) {
+  // one row of this group: its piece in `r`, the piece's address (PAIR_MEMORY) in `row`
+  auto turn_row = [&](uint4 r, const elem16 *row, const float (&A)[8], const float (&B)[8]) {
     float x[8], z[8];
     unpack8<F16>(r, x);
     float inv = 1.f;
-    if (norm) {
+    if (weight) {
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
@@ -198,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __gr
       unpack8<F16>(o, z);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++) z[i] = in_row && e0 + i < dims ? elem_value<F16>(src[partner(e0 + i) - e0]) : 0.f;
+      for (int i = 0; i < 8; i++) z[i] = in_row && e0 + i < dims ? elem_value<F16>(row[partner(e0 + i) - e0]) : 0.f;
       __syncwarp(lanes);  // the row may be rotated in place: all of it has been read
     }
     uint32_t out[4];
@@ -208,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __gr
     return make_uint4(out[0], out[1], out[2], out[3]);
   };
   for (;;) {
-    if (tok < n_tok) {
+    if (tok < n_tok && first < n_heads) {
       // Sine and cosine for this lane's elements.  The phase's top word is within half a turn, where
       // the hardware's sine and cosine are off by at most 2^-20.9 absolute: nothing against the
       // half step of 2^-9 or 2^-12 that the result is rounded by.
@@ -233,124 +223,166 @@ __global__ void __launch_bounds__(kThreads, 3) rope_norm_cache_kernel(const __gr
           B[i] = on ? (e0 + i < half ? -sn : sn) : 0.f;
         }
       }
-      if (first == share - 1) {  // the key row
-        float Ak[8], Bk[8];
+      if (weight && in_row) {  // A *= w, B *= the partner's w
+        float w[8];
+        unpack8<F16>(*reinterpret_cast<const uint4 *>(weight + e0), w);
 #pragma unroll
-        for (int i = 0; i < 8; i++) Ak[i] = A[i], Bk[i] = B[i];
-        if (p.k_norm_w && in_row) weigh(p.k_norm_w, Ak, Bk);
-        const uint4 out = turn_row(raw_k, p.k + t * p.k_stride + h * D + e0, p.k_norm_w != nullptr, Ak, Bk);
-        if (in_row) {
-          if (p.k_out) *reinterpret_cast<uint4 *>(p.k_out + t * p.k_out_stride + h * D + e0) = out;
-          if (write && FP8) {
-            const uint2 q8 = quantise8<F16>(out, p.k_scale);
-            if (has_exponent15(q8) && p.slot_mapping[t] >= 0) atomicOr(p.special, 1u);
-            *reinterpret_cast<uint2 *>(k_s + tok * D + e0) = q8;
-          } else if (write) {
-            *reinterpret_cast<uint4 *>(k_s + (tok * D + e0) * 2) = out;
-          }
+        for (int i = 0; i < 8; i++) A[i] *= w[i];
+        if (PAIR == PAIR_LANE) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) B[i] *= w[i ^ 1];
+        } else if (PAIR == PAIR_SHUFFLE) {
+          unpack8<F16>(*reinterpret_cast<const uint4 *>(weight + other * 8), w);
+#pragma unroll
+          for (int i = 0; i < 8; i++) B[i] *= w[i];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+            if (e0 + i < dims) B[i] *= elem_value<F16>(weight[partner(e0 + i)]);
         }
       }
-      if (p.q_norm_w && in_row) weigh(p.q_norm_w, A, B);
-      elem16 *const q_dst = p.q_out + t * p.q_out_stride + (int64_t)h * G * D + e0;
-      for (int base = first; base < G; base += BATCH << share_log) {
-        if (base != first) load_q(base);
+      elem16 *const dst = keys ? p.k_out ? p.k_out + t * p.k_out_stride + (int64_t)h * D + e0 : nullptr
+                               : p.q_out + t * p.q_out_stride + (int64_t)h * D + e0;
+      for (int base = first; base < n_heads; base += BATCH << share_log) {
+        if (base != first) load_rows(base);
 #pragma unroll
         for (int b = 0; b < BATCH; b++) {
           const int r = base + (b << share_log);
-          if (r >= G) break;
-          const uint4 out = turn_row(raw[b], q_src + r * D, p.q_norm_w != nullptr, A, B);
-          if (in_row) *reinterpret_cast<uint4 *>(q_dst + r * D) = out;
+          if (r >= n_heads) break;
+          const uint4 out = turn_row(raw[b], src + r * D, A, B);
+          if (in_row && dst) *reinterpret_cast<uint4 *>(dst + r * D) = out;
+          if (in_row && write) {
+            uint8_t *st = k_s + ((r * tokens + tok) * D + e0) * kElem;
+            if (FP8) {
+              const uint2 q8 = quantise8<F16>(out, p.k_scale);
+              if (has_exponent15(q8) && p.slot_mapping[t] >= 0) atomicOr(p.special, 1u);
+              *reinterpret_cast<uint2 *>(st) = q8;
+            } else {
+              *reinterpret_cast<uint4 *>(st) = out;
+            }
+          }
         }
       }
     }
     // fewer groups than tokens (rows of 32 lanes): a group takes a second token
     tok += kGroups;
     if (tok >= tokens) break;
-    load_token();
+    src = x_in + tok * x_stride;
+    load_rows(first);
   }
   if (!write) return;
+  if (!FP8) asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
 
   // ---- pool write, token index fastest across threads: a thread keeps its token ----------------
   const int wt = tid & (tokens - 1), bs = 1 << p.bs_log;
   const int64_t slot = slot_s[wt];
   const int off = (int)(slot & (bs - 1));
-  const int64_t chunk = (((slot >> p.bs_log) * p.Hkv + h) * (int64_t)D << p.bs_log) * kElem;  // bytes
-  if (slot >= 0) {
-    uint8_t *dst = static_cast<uint8_t *>(p.k_pool) + chunk + off * 16;
-    for (int c = tid >> tok_log; c < D * kElem / 16; c += kThreads >> tok_log)
-      *reinterpret_cast<uint4 *>(dst + c * bs * 16) = *reinterpret_cast<const uint4 *>(k_s + wt * D * kElem + c * 16);
-  }
+  const int chunk_bytes = (D << p.bs_log) * kElem;
+  const int64_t chunk0 = ((slot >> p.bs_log) * p.Hkv + h) * (int64_t)chunk_bytes;
   // an aligned run of 16 slots (two blocks of 8 tokens are not one)
   const bool run = __all_sync(0xffffffffu, tokens == kTokMax && bs >= kTokMax && slot >= 0 && slot == slot_s[0] + wt && (slot_s[0] & 15) == 0);
   const int warp = tid >> 5, lane = tid & 31;
+  if (slot >= 0) {
+    uint8_t *const dst = static_cast<uint8_t *>(p.k_pool) + chunk0 + off * 16;
+    for (int r = 0; r < n_heads; r++)
+      for (int c = tid >> tok_log; c < D * kElem / 16; c += kThreads >> tok_log)
+        *reinterpret_cast<uint4 *>(dst + r * chunk_bytes + c * bs * 16) =
+            *reinterpret_cast<const uint4 *>(k_s + (r * tokens + wt) * D * kElem + c * 16);
+  }
+  uint8_t *const v_dst = static_cast<uint8_t *>(p.v_pool) + chunk0;
   if (run && !FP8) {
     // matrices 0 and 1 hold 8 dimensions, 2 and 3 the next 8; row r of matrix m is token
     // (r / 2) * 4 + 2 (m % 2) + r % 2, so that a lane ends up with four tokens of a dimension
-    const int m = lane >> 3, r = lane & 7, mt = (r >> 1) * 4 + (m & 1) * 2 + (r & 1);
-    const int64_t run_at = chunk + (slot_s[0] & (bs - 1)) * 2;
-    for (int d0 = warp * 16; d0 < D; d0 += kThreads / 2) {
-      uint32_t w[4];
-      ldmatrix_x4_trans(w, smem_u32(v_s) + mt * v_row + (d0 + (m >> 1) * 8) * 2);
-      uint8_t *dst = static_cast<uint8_t *>(p.v_pool) + run_at + (lane & 3) * 8;
-      const int d = d0 + (lane >> 2);
-      *reinterpret_cast<uint2 *>(dst + (int64_t)d * bs * 2) = make_uint2(w[0], w[1]);
-      if (d + 8 < D) *reinterpret_cast<uint2 *>(dst + (int64_t)(d + 8) * bs * 2) = make_uint2(w[2], w[3]);
-    }
+    const int m = lane >> 3, mr = lane & 7, mt = (mr >> 1) * 4 + (m & 1) * 2 + (mr & 1);
+    const int run_off = (int)(slot_s[0] & (bs - 1)) * 2 + (lane & 3) * 8;
+    for (int r = 0; r < n_heads; r++)
+      for (int d0 = warp * 16; d0 < D; d0 += kThreads / 2) {
+        uint32_t w[4];
+        ldmatrix_x4_trans(w, smem_u32(v_s) + (r * tokens + mt) * v_row + (d0 + (m >> 1) * 8) * 2);
+        uint8_t *dst = v_dst + r * chunk_bytes + run_off;
+        const int d = d0 + (lane >> 2);
+        *reinterpret_cast<uint2 *>(dst + d * bs * 2) = make_uint2(w[0], w[1]);
+        if (d + 8 < D) *reinterpret_cast<uint2 *>(dst + (d + 8) * bs * 2) = make_uint2(w[2], w[3]);
+      }
   } else if (run) {
     // four tokens x four dimensions of bytes per thread
-    if (tid < D) {
-      const int tq = tid & 3, d = (tid >> 2) * 4;
+    for (int i = tid; i < n_heads * D; i += kThreads) {
+      const int r = i / kHeadSize, tq = i & 3, d = (i % kHeadSize >> 2) * 4;  // FP8 caches have head size 128
       uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint32_t *>(v_s + (tq * 4 + i) * v_row + d);
+      for (int k = 0; k < 4; k++) w[k] = *reinterpret_cast<const uint32_t *>(v_s + (r * tokens + tq * 4 + k) * v_row + d);
       const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);  // dimensions 0, 1
       const uint32_t c = __byte_perm(w[0], w[1], 0x7362), e = __byte_perm(w[2], w[3], 0x7362);  // dimensions 2, 3
-      uint8_t *dst = static_cast<uint8_t *>(p.v_pool) + chunk + (slot_s[0] & (bs - 1)) + tq * 4 + d * bs;
+      uint8_t *dst = v_dst + r * chunk_bytes + (int)(slot_s[0] & (bs - 1)) + tq * 4 + d * bs;
       *reinterpret_cast<uint32_t *>(dst) = __byte_perm(a, b, 0x5410);
       *reinterpret_cast<uint32_t *>(dst + bs) = __byte_perm(a, b, 0x7632);
       *reinterpret_cast<uint32_t *>(dst + 2 * bs) = __byte_perm(c, e, 0x5410);
       *reinterpret_cast<uint32_t *>(dst + 3 * bs) = __byte_perm(c, e, 0x7632);
     }
   } else if (slot >= 0) {
-    for (int d = tid >> tok_log; d < D; d += kThreads >> tok_log) {
-      if (FP8) static_cast<uint8_t *>(p.v_pool)[chunk + d * bs + off] = v_s[wt * v_row + d];
-      else static_cast<elem16 *>(p.v_pool)[chunk / 2 + d * bs + off] = *reinterpret_cast<const elem16 *>(v_s + wt * v_row + d * 2);
-    }
+    for (int r = 0; r < n_heads; r++)
+      for (int d = tid >> tok_log; d < D; d += kThreads >> tok_log) {
+        const uint8_t *from = v_s + (r * tokens + wt) * v_row + d * kElem;
+        uint8_t *to = v_dst + r * chunk_bytes + (d * bs + off) * kElem;
+        if (FP8) *to = *from;
+        else *reinterpret_cast<elem16 *>(to) = *reinterpret_cast<const elem16 *>(from);
+      }
   }
 }
 
+// Heads of a CTA and the grid for `tokens` tokens to a CTA.
+struct Shape {
+  int q_heads, kv_heads, kv_ctas;
+  dim3 grid;
+  size_t smem;
+};
+Shape shape_of(const RotateParams &p, int tok_log, bool fp8) {
+  const int tokens = 1 << tok_log, gw = p.D <= 32 ? 4 : p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32;
+  const int share = std::max((kThreads / gw) >> tok_log, 1);  // groups of a token
+  const int head_bytes = tokens * (p.D * (fp8 ? 2 : 4) + 16);
+  Shape s;
+  s.q_heads = std::min(p.Hq, std::max(16, share));
+  s.kv_heads = std::max(1, std::min({p.Hkv, std::max(4, share), 40960 / head_bytes}));
+  s.kv_ctas = (p.Hkv + s.kv_heads - 1) / s.kv_heads;
+  s.grid = dim3((unsigned)((p.num_tokens + tokens - 1) >> tok_log), (unsigned)(s.kv_ctas + (p.Hq + s.q_heads - 1) / s.q_heads));
+  s.smem = (size_t)s.kv_heads * head_bytes;
+  return s;
+}
+
 template <int GW, bool FP8, bool F16, int PAIR>
-cudaError_t launch_pair(const RotateParams &p, int tok_log, dim3 grid, size_t smem, cudaStream_t st) {
-  const int G = p.Hq / p.Hkv, share = (kThreads / GW) >> tok_log;  // groups of a token
-  if (share >= G) rope_norm_cache_kernel<GW, F16, FP8, PAIR, 1><<<grid, kThreads, smem, st>>>(p, tok_log, G);
-  else rope_norm_cache_kernel<GW, F16, FP8, PAIR, 4><<<grid, kThreads, smem, st>>>(p, tok_log, G);
+cudaError_t launch_pair(const RotateParams &p, int tok_log, cudaStream_t st) {
+  const Shape s = shape_of(p, tok_log, FP8);
+  const int share = (kThreads / GW) >> tok_log;
+  auto go = [&](auto kernel) { kernel<<<s.grid, kThreads, s.smem, st>>>(p, tok_log, s.q_heads, s.kv_heads, s.kv_ctas); };
+  if (share >= s.q_heads && share >= s.kv_heads) go(rope_norm_cache_kernel<GW, F16, FP8, PAIR, 1>);
+  else go(rope_norm_cache_kernel<GW, F16, FP8, PAIR, 4>);
   return cudaGetLastError();
 }
 template <int GW, bool FP8, bool F16>
-cudaError_t launch_group(const RotateParams &p, int tok_log, dim3 grid, size_t smem, cudaStream_t st) {
-  if (p.rope.interleaved) return launch_pair<GW, FP8, F16, PAIR_LANE>(p, tok_log, grid, smem, st);
-  if (p.rope.dims % 16 == 0) return launch_pair<GW, FP8, F16, PAIR_SHUFFLE>(p, tok_log, grid, smem, st);
-  return launch_pair<GW, FP8, F16, PAIR_MEMORY>(p, tok_log, grid, smem, st);
+cudaError_t launch_group(const RotateParams &p, int tok_log, cudaStream_t st) {
+  if (p.rope.interleaved) return launch_pair<GW, FP8, F16, PAIR_LANE>(p, tok_log, st);
+  if (p.rope.dims % 16 == 0) return launch_pair<GW, FP8, F16, PAIR_SHUFFLE>(p, tok_log, st);
+  return launch_pair<GW, FP8, F16, PAIR_MEMORY>(p, tok_log, st);
 }
 
 }  // namespace
 
 cudaError_t launch_rope_norm_cache(const RotateParams &p, bool f16, bool fp8, int num_sms, cudaStream_t st) {
   if (p.num_tokens <= 0) return cudaSuccess;
-  // about two CTAs per SM before a CTA takes more than one token
-  int tok_log = 0;
-  while (tok_log < 4 && (p.num_tokens * p.Hkv >> (tok_log + 1)) >= 2 * num_sms) tok_log++;
-  const int tokens = 1 << tok_log;
-  const dim3 grid((unsigned)((p.num_tokens + tokens - 1) >> tok_log), (unsigned)p.Hkv);
-  const size_t smem = (size_t)tokens * (p.D * (fp8 ? 2 : 4) + 16);
+  // two CTAs per SM before a CTA takes more than one token
+  int tok_log = 4;
+  for (; tok_log > 0; tok_log--) {
+    const Shape s = shape_of(p, tok_log, fp8);
+    if ((int64_t)s.grid.x * s.grid.y >= 2 * num_sms) break;
+  }
   auto go = [&](auto f16_tag) {
     constexpr bool F16 = decltype(f16_tag)::value;
-    if (fp8) return launch_group<16, true, F16>(p, tok_log, grid, smem, st);
-    if (p.D <= 32) return launch_group<4, false, F16>(p, tok_log, grid, smem, st);
-    if (p.D <= 64) return launch_group<8, false, F16>(p, tok_log, grid, smem, st);
-    if (p.D <= 128) return launch_group<16, false, F16>(p, tok_log, grid, smem, st);
-    return launch_group<32, false, F16>(p, tok_log, grid, smem, st);
+    if (fp8) return launch_group<16, true, F16>(p, tok_log, st);
+    if (p.D <= 32) return launch_group<4, false, F16>(p, tok_log, st);
+    if (p.D <= 64) return launch_group<8, false, F16>(p, tok_log, st);
+    if (p.D <= 128) return launch_group<16, false, F16>(p, tok_log, st);
+    return launch_group<32, false, F16>(p, tok_log, st);
   };
   const cudaError_t e = f16 ? go(std::true_type{}) : go(std::false_type{});
   __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
