@@ -253,6 +253,33 @@ def test_rotate_fp8_overflow_switches_the_cache_to_exact(cuda_device):
         assert not torch.isfinite(out[0, :, 7]).any()
 
 
+@pytest.mark.parametrize("f16", [False, True])
+def test_rotate_fp8_bytes_of_every_element(cuda_device, f16):
+    """Every 16-bit pattern, under scales that divide exactly and scales that do not: the bytes of
+    the plain cache write, which are pinned to the oracle elsewhere."""
+    t = T16[f16]
+    bits = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(t)
+    x = bits[torch.randperm(65536, generator=gen(1), device="cuda")].view(256, 2, 128)
+    x = torch.cat((x, bits.view(256, 2, 128)))  # mixed and sorted neighbours
+    n = x.shape[0]
+    slots = torch.arange(n, device="cuda")
+    pos = torch.zeros(n, dtype=torch.int32, device="cuda")
+    q = torch.zeros(n, 2, 128, dtype=t, device="cuda")
+    plan = pa.RopePlan(2, 1e4)
+    for ks, vs in ((1.0, 0.0371), (1 / 16, 3.0), (1e-3, 7e4), (1e-30, 1e30), (1.1, 0.9999999), (2.0 ** -61, 2.0 ** 61)):
+        pools = [torch.zeros(n // 16, 2, 8, 16, 16, dtype=torch.uint8, device="cuda") for _ in range(4)]
+        caches = []
+        for i in (0, 2):
+            caches.append(pa.PagedCache(16, n // 16, 128, 2, dtype=0 if f16 else 1, key_pools=pools[i:i + 1],
+                                        value_pools=pools[i + 1:i + 2], fp8=True))
+            caches[-1].set_kv_scales(ks, vs)
+        k_out = torch.empty_like(x)
+        caches[0].rope_norm_and_cache(plan, q, k_out, q, x, x, None, None, 0.0, pos, slots, n, 2)
+        caches[1].reshape_and_cache(k_out, x, slots, n, 256, 256)
+        torch.cuda.synchronize()
+        assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3]), (ks, vs)
+
+
 def test_rotate_special_values(cuda_device):
     """NaN and infinity stay in their row and pair; a zero row stays zero."""
     r = Rotate(20, 4, 2, 128, 128, norm=False, seed=4)
