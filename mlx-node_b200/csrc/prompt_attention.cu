@@ -4,8 +4,9 @@
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i k_j - m_i),  j <= kv_len - q_len + i
 //
 // with m_i any number near the row's largest logit (it cancels).  One pass over the keys: the
-// running maximum and sum are kept in fp32 per row; the maximum is stale - it moves only when
-// a logit exceeds it by more than 2^8 - so that the accumulator is rarely rescaled.
+// running maximum and sum are kept in fp32 per row.  The maximum is stale: a tile's probabilities
+// are taken against the maximum of the tiles before it, and it moves - before the next tile - only
+// when a logit exceeded it by more than 2^8, so that the accumulator is rarely rescaled.
 // Probabilities are rounded to the 16-bit type because the tensor cores take both operands of
 // P.V in one 16-bit type; their sum is taken before the rounding.
 //
@@ -20,7 +21,9 @@
 // Roles (warps):
 //   8 per query tile  softmax: two threads per row, each 64 of a tile's 128 logits, so that a
 //                     scheduler has two warps of a tile in flight while the other query tile
-//                     is in the tensor cores
+//                     is in the tensor cores.  The two tell each other their maxima through
+//                     shared memory and read them a tile later, when the barriers of the P.V in
+//                     between have ordered them: no barrier of their own
 //   1                 copies: Q per item, K and V tiles into two rings
 //   1                 issues every tcgen05.mma (two more idle: register budgets move between
 //                     warpgroups of four)
@@ -65,7 +68,8 @@ struct Geo {
                        B_PVDONE = B_PREADY + QT, kBars = B_PVDONE + QT;
   static constexpr int kXch = 2 * QT * 2 * 128 * 4;     // [parity][query tile][half][row] floats
   static constexpr int kWalk = kThreads / 32 * 16;       // a PlanPos per warp
-  static constexpr int kSmem = 1024 + (QT + NK + NV) * kTile + kXch + kWalk + kBars * 8 + 16;
+  static constexpr int kWords = 8 * QT * 4;             // a meeting word per softmax warp
+  static constexpr int kSmem = 1024 + (QT + NK + NV) * kTile + kXch + kWalk + kWords + kBars * 8 + 16;
   static_assert(kSmem <= 232448, "shared memory per CTA");
 };
 
@@ -136,6 +140,12 @@ __device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
                  "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]),
                  "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
 
@@ -230,6 +240,93 @@ __device__ __noinline__ bool masked_value_not_finite(const PromptParams &p, int 
   return __any_sync(0xffffffffu, bad);
 }
 
+// The rare case that a logit of the current tile is so far above the stale maximum that its
+// probability would leave the 16-bit type's (f16) or the accumulator's comfortable range: the two
+// warps of a set of rows meet and settle on the tile's own maximum before the tile's P.V may start.
+// One of them found the case before it stored its probabilities and takes them again from the
+// logits; the other may have stored and announced its own (`stored`) and scales those.  Neither
+// can run ahead: P.V waits for the first one's announcement.  The meetings are words in shared
+// memory with a bounded wait, so that a CTA that has given up elsewhere does not hang here.
+struct Redo {
+  float m_used, l, sum;
+};
+__device__ __forceinline__ void redo_meet(uint32_t mine, uint32_t other, uint32_t stamp, volatile int *abort_flag) {
+  __threadfence_block();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(mine), "r"(stamp) : "memory");
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t w;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(w) : "r"(other) : "memory");
+    if (__all_sync(0xffffffffu, (int)(w - stamp) >= 0 || *abort_flag)) break;
+    if (clock64() - t0 > (1ll << 31)) *abort_flag = 1;
+  }
+  __threadfence_block();
+  __syncwarp();
+}
+template <bool CAP, bool F16>
+__device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int half, float c, float cap_in, float cap_out, float m_used,
+                                       float l, float mx, uint32_t mx_other, uint32_t word_mine, uint32_t word_other,
+                                       uint32_t stamp, bool valid, bool stored, bool rescale, int left,
+                                       volatile int *abort_flag) {
+  redo_meet(word_mine, word_other, stamp, abort_flag);
+  float theirs;
+  asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(theirs) : "r"(mx_other) : "memory");
+  const float m_new = fmaxf(m_used, fmaxf(mx, theirs));
+  float factor = 1.f;
+  if (valid && m_new > m_used) {
+    factor = m_used == -INFINITY ? 0.f : fast_exp2((m_used - m_new) * c);
+    m_used = m_new;
+  }
+  if (rescale) {
+    for (int ch = half; ch * 32 < D; ch += 2) {
+      uint32_t r[32];
+      tmem_ld32(o_t + ch * 32, r);
+      tmem_wait_ld32(r);
+#pragma unroll
+      for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
+      tmem_st32(o_t + ch * 32, r);
+    }
+  }
+  float sum = 0.f;
+  if (stored) {
+    uint32_t r[32];
+    tmem_ld32(s_t, r);
+    tmem_wait_ld32(r);
+#pragma unroll
+    for (int e = 0; e < 32; e++)
+      r[e] = pack2<F16>(elem_value<F16>(r[e] & 0xffffu) * factor, elem_value<F16>(r[e] >> 16) * factor);
+    tmem_st32(s_t, r);
+  } else {
+    const float mc = m_used == -INFINITY ? 0.f : m_used * c;
+#pragma unroll 1
+    for (int ch = 0; ch < 4; ch++) {
+      uint32_t r[16];
+      tmem_ld16(s_t + ch * 16, r);
+      tmem_wait_ld16(r);
+      uint32_t t[8];
+#pragma unroll
+      for (int e = 0; e < 16; e++) {
+        float x = __uint_as_float(r[e]);
+        if (CAP) x = tanhf(x * cap_in) * cap_out;
+        if (ch * 16 + e >= left) x = -INFINITY;
+        const float pe = fast_exp2(fmaf(x, c, -mc));
+        sum += pe;
+        r[e] = __float_as_uint(pe);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) t[e] = pack2<F16>(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1]));
+      // columns that have been read already: chunk ch goes over logits 8 ch .. 8 ch + 7
+      tmem_st8(s_t + ch * 8, t);
+    }
+  }
+  tmem_wait_st();
+  tc_fence_before();
+  redo_meet(word_mine, word_other, stamp + 1, abort_flag);
+  tc_fence_after();
+  return Redo{m_used, l * factor, sum};
+}
+
 template <int NBOX, bool CAP, bool F16>
 __global__ void __launch_bounds__(Geo<NBOX>::kThreads, 1)
 prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_constant__ CUtensorMap q_map,
@@ -241,7 +338,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
   const uint32_t q_s = base, k_s = q_s + Z::QT * Z::kTile, v_s = k_s + Z::NK * Z::kTile;
   float *xch = reinterpret_cast<float *>(gen + (Z::QT + Z::NK + Z::NV) * Z::kTile);
   PlanPos *const at = reinterpret_cast<PlanPos *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch) + (threadIdx.x >> 5);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch + Z::kWalk);
+  uint32_t *const words = reinterpret_cast<uint32_t *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch + Z::kWalk);
+  uint64_t *bars = reinterpret_cast<uint64_t *>(words + 8 * Z::QT);
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Z::kBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
@@ -259,6 +357,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       mbar_init(bar(Z::B_PREADY + i), 8);
       mbar_init(bar(Z::B_PVDONE + i), 1);
     }
+    for (int i = 0; i < 8 * Z::QT; i++) words[i] = 0;
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -396,18 +495,42 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     const uint32_t o_t = tmem + lane_base + 256 + i * 128;
     const int sync_id = 1 + i * 4 + quad;  // the two warps that share these rows
     const uint32_t mine = smem_u32(xch) + ((i * 2 + half) * 128 + row) * 4;
-    uint32_t xc = 0;   // exchanges so far: two slots in turn
-    uint32_t cnt = 0;  // logit tiles seen
+    const uint32_t theirs = mine + (half ? -512 : 512);
+    constexpr uint32_t kSlot = Z::QT * 2 * 128 * 4;
+    const uint32_t word_mine = smem_u32(words + warp), word_other = smem_u32(words + (warp ^ 4));
+    uint32_t cnt = 0;  // logit tiles seen; the maxima of tile n are in slot n & 1
     const float c = p.scale * kLog2e;
     // soft-capping: x -> tanh(x*scale/cap)*cap/scale, so that x*c is the capped logit
     const float cap_in = p.scale / p.softcap, cap_out = p.softcap / p.scale;
-    auto exchange = [&](float x) {
-      const uint32_t a = mine + (xc++ & 1) * (Z::QT * 2 * 128 * 4), b = a + (half ? -512 : 512);
+    // Probabilities of up to 2^kFar against the stale maximum are taken as they are: f16 ends at 2^16,
+    // bf16 and the fp32 sums have room for any that this leaves.
+    constexpr float kFar = F16 ? 15.f : 40.f;
+    auto put = [&](uint32_t slot, float x) { asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(mine + slot * kSlot), "f"(x) : "memory"); };
+    auto get = [&](uint32_t slot) {
       float y;
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(x) : "memory");
-      pair_sync(sync_id);
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(b) : "memory");
+      asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(y) : "r"(theirs + slot * kSlot) : "memory");
       return y;
+    };
+    // Waits for a barrier that cannot complete before both warps of these rows have announced tile
+    // cnt - 1; meanwhile the other one may call for a meeting about that tile (redo_tile).
+    auto wait_pending = [&](uint32_t b, uint32_t parity, auto &&join) {
+      if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return;
+      const long long t0 = clock64();
+      bool met = false;
+      while (!__all_sync(0xffffffffu, mbar_try_wait(b, parity))) {
+        uint32_t w;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(w) : "r"(word_other) : "memory");
+        if (!met && __any_sync(0xffffffffu, w == 2 * cnt)) {
+          join();
+          met = true;
+        }
+        if (*abort_flag) failed = true;
+        if (clock64() - t0 > (1ll << 31)) failed = true, *abort_flag = 1;
+        if (__any_sync(0xffffffffu, failed)) {
+          failed = true;
+          return;
+        }
+      }
     };
     // After a wait that ran out these warps keep going through the motions (every further wait
     // returns at once): two of them share each row's barrier, and one that left would leave
@@ -420,14 +543,29 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       int min_lim = lim;
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, o));
-      float m_used = -INFINITY, l = 0.f;
+      float m_used = -INFINITY, l = 0.f, mx = -INFINITY;
+      bool behind = false;  // tile cnt - 1 belongs to this item and its meeting, if any, may be ahead
+      int left = 0;         // columns of the tile from here on are masked
+      auto redo = [&](bool stored, bool rescale) {
+        const uint32_t tile = stored ? cnt - 1 : cnt;
+        const Redo r = redo_tile<CAP, F16>(s_t, o_t, D, half, c, cap_in, cap_out, m_used, l, mx, theirs + (tile & 1) * kSlot, word_mine,
+                                           word_other, 2 * (tile + 1), valid, stored, rescale, left, abort_flag);
+        m_used = r.m_used;
+        l = r.l;
+        return r.sum;
+      };
       for (int t = g.kt0; t < g.kt1; t++, cnt++) {
-        failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
-        __syncwarp();
+        const bool first = t == g.kt0;
+        if (first) {
+          failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
+          __syncwarp();
+        } else {
+          wait_pending(bar(Z::B_SFULL + i), cnt & 1, [&] { behind ? (void)redo(true, t > g.kt0 + 1) : (void)0; });
+        }
         tc_fence_after();
         const int key0 = t * kKeyTile + half * 64;
         const bool need_mask = key0 + 64 > min_lim;
-        const int left = lim - key0;  // columns from here on are masked
+        left = lim - key0;
         auto cap_and_mask = [&](uint32_t (&r)[16], int col0) {
           if (CAP) {
 #pragma unroll
@@ -439,12 +577,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
               if (col0 + e >= left) r[e] = 0xff800000u;
           }
         };
-        float mx, sum;
-        uint32_t pr[32];  // the row half's probabilities, packed
-        bool settled = t == g.kt0;
-        if (settled) {  // the first tile sets the reference
+        if (first) {  // the first tile sets the reference
           mx = -INFINITY;
-#pragma unroll
+#pragma unroll 1
           for (int ch = 0; ch < 4; ch++) {
             uint32_t r[16];
             tmem_ld16(s_t + ch * 16, r);
@@ -453,9 +588,36 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
           }
-          m_used = fmaxf(mx, exchange(mx));
+          put(cnt & 1, mx);
+          pair_sync(sync_id);
+          m_used = fmaxf(mx, get(cnt & 1));
+          pair_sync(sync_id);  // both have read: the tile's own maxima go to the same place below
+        } else {
+          // both halves of a row see the same maximum of the tile before and decide alike
+          mx = fmaxf(mx, get((cnt - 1) & 1));
+          const bool grew = valid && mx > m_used && !((mx - m_used) * c <= 8.f);
+          if (__any_sync(0xffffffffu, grew)) {
+            float factor = 1.f;
+            if (grew) {
+              factor = m_used == -INFINITY ? 0.f : fast_exp2((m_used - mx) * c);
+              m_used = mx;
+            }
+            // O holds the tiles before this one: S of this tile was issued after their P.V
+#pragma unroll 1
+            for (int ch = half; ch * 32 < D; ch += 2) {
+              uint32_t r[32];
+              tmem_ld32(o_t + ch * 32, r);
+              tmem_wait_ld32(r);
+#pragma unroll
+              for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
+              tmem_st32(o_t + ch * 32, r);
+            }
+            l *= factor;
+          }
         }
-        for (;;) {
+        float sum;
+        uint32_t pr[32];  // the row half's probabilities, packed
+        {
           const float mc = m_used == -INFINITY ? 0.f : m_used * c;
           float mxa[2] = {-INFINITY, -INFINITY}, sma[4] = {0.f, 0.f, 0.f, 0.f};
           // 16 columns at a time, the next 16 on their way from TMEM meanwhile
@@ -486,32 +648,18 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           part_pass(b, 3);
           mx = fmaxf(mxa[0], mxa[1]);
           sum = (sma[0] + sma[1]) + (sma[2] + sma[3]);
-          if (settled) break;
-          // both halves of a row see the same maximum and decide alike
-          mx = fmaxf(mx, exchange(mx));
-          const bool grew = valid && mx > m_used && !((mx - m_used) * c <= 8.f);
-          if (!__any_sync(0xffffffffu, grew)) break;
-          float factor = 1.f;
-          if (grew) {
-            factor = m_used == -INFINITY ? 0.f : fast_exp2((m_used - mx) * c);
-            m_used = mx;
-          }
-          // O holds the tiles before this one: S of this tile was issued after their P.V
-          for (int ch = half; ch * 32 < D; ch += 2) {
-            uint32_t r[32];
-            tmem_ld32(o_t + ch * 32, r);
-            tmem_wait_ld32(r);
-#pragma unroll
-            for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
-            tmem_st32(o_t + ch * 32, r);
-          }
-          l *= factor;
-          settled = true;  // the logits are still in TMEM: once more against the new reference
+        }
+        put(cnt & 1, mx);
+        behind = true;
+        if (__any_sync(0xffffffffu, valid && (mx - m_used) * c > kFar)) {
+          sum = redo(false, !first);
+          behind = false;
+        } else {
+          tmem_st32(s_t, pr);
+          tmem_wait_st();
+          tc_fence_before();
         }
         l += sum;
-        tmem_st32(s_t, pr);
-        tmem_wait_st();
-        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(Z::B_PREADY + i));
       }
@@ -524,11 +672,16 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             for (int e = ch * 32; e < D && e < ch * 32 + 32; e += 8) *reinterpret_cast<uint4 *>(orow + e) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      const float l_other = exchange(l);
-      l = half == 0 ? l + l_other : l_other + l;
-      failed |= !wait_bar(bar(Z::B_PVDONE + i), (cnt - 1) & 1, abort_flag);
-      __syncwarp();
+      wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] { behind ? (void)redo(true, g.kt1 > g.kt0 + 1) : (void)0; });
       tc_fence_after();
+      pair_sync(sync_id);  // both are through with the maxima
+      put(0, l);
+      pair_sync(sync_id);
+      {
+        const float l_other = get(0);
+        l = half == 0 ? l + l_other : l_other + l;
+      }
+      pair_sync(sync_id);
       const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
       constexpr int kRows = 128 * Z::QT;
       float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 2) * kRows + i * 128 + row;
