@@ -3,10 +3,12 @@
 //
 //   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i k_j - m_i),  j <= kv_len - q_len + i
 //
-// with m_i any number near the row's largest logit (it cancels).  One pass over the keys: the
-// running maximum and sum are kept in fp32 per row.  The maximum is stale: a tile's probabilities
-// are taken against the maximum of the tiles before it, and it moves - before the next tile - only
-// when a logit exceeded it by more than 2^8, so that the accumulator is rarely rescaled.
+// with m_i any number near the row's largest logit (it cancels).  One pass over the keys: reference
+// and running sum are kept in fp32 per row, the reference in units of log2.  It is the maximum of
+// the first tile, and stale after that: a tile's probabilities are taken against the reference of
+// the tiles before it, and it moves - before the next tile - only when the tile's sum of
+// probabilities exceeded 2^8, by log2 of that sum, which is the tile's maximum plus seven at most.
+// So no maximum is taken in the loop, and the accumulator is rarely rescaled.
 // Probabilities are rounded to the 16-bit type because the tensor cores take both operands of
 // P.V in one 16-bit type; their sum is taken before the rounding.
 //
@@ -21,7 +23,7 @@
 // Roles (warps):
 //   8 per query tile  softmax: two threads per row, each 64 of a tile's 128 logits, so that a
 //                     scheduler has two warps of a tile in flight while the other query tile
-//                     is in the tensor cores.  The two tell each other their maxima through
+//                     is in the tensor cores.  The two tell each other their sums through
 //                     shared memory and read them a tile later, when the barriers of the P.V in
 //                     between have ordered them: no barrier of their own
 //   1                 copies: Q per item, K and V tiles into two rings
@@ -240,15 +242,15 @@ __device__ __noinline__ bool masked_value_not_finite(const PromptParams &p, int 
   return __any_sync(0xffffffffu, bad);
 }
 
-// The rare case that a logit of the current tile is so far above the stale maximum that its
-// probability would leave the 16-bit type's (f16) or the accumulator's comfortable range: the two
-// warps of a set of rows meet and settle on the tile's own maximum before the tile's P.V may start.
-// One of them found the case before it stored its probabilities and takes them again from the
-// logits; the other may have stored and announced its own (`stored`) and scales those.  Neither
-// can run ahead: P.V waits for the first one's announcement.  The meetings are words in shared
-// memory with a bounded wait, so that a CTA that has given up elsewhere does not hang here.
+// The rare case that a logit of the current tile is so far above the reference that its probability
+// would leave the 16-bit type's (f16) or the accumulator's comfortable range: the two warps of a set
+// of rows meet and settle on the tile's own maximum before the tile's P.V may start.  One of them
+// found the case before it stored its probabilities and takes them again from the logits; the other
+// may have stored and announced its own (`stored`) and scales those.  Neither can run ahead: P.V
+// waits for the first one's announcement.  The meetings are words in shared memory with a bounded
+// wait, so that a CTA that has given up elsewhere does not hang here.
 struct Redo {
-  float m_used, l, sum;
+  float ref, l, sum;
 };
 __device__ __forceinline__ void redo_meet(uint32_t mine, uint32_t other, uint32_t stamp, volatile int *abort_flag) {
   __threadfence_block();
@@ -264,31 +266,57 @@ __device__ __forceinline__ void redo_meet(uint32_t mine, uint32_t other, uint32_
   __threadfence_block();
   __syncwarp();
 }
-template <bool CAP, bool F16>
-__device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int half, float c, float cap_in, float cap_out, float m_used,
-                                       float l, float mx, uint32_t mx_other, uint32_t word_mine, uint32_t word_other,
-                                       uint32_t stamp, bool valid, bool stored, bool rescale, int left,
-                                       volatile int *abort_flag) {
-  redo_meet(word_mine, word_other, stamp, abort_flag);
-  float theirs;
-  asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(theirs) : "r"(mx_other) : "memory");
-  const float m_new = fmaxf(m_used, fmaxf(mx, theirs));
-  float factor = 1.f;
-  if (valid && m_new > m_used) {
-    factor = m_used == -INFINITY ? 0.f : fast_exp2((m_used - m_new) * c);
-    m_used = m_new;
-  }
-  if (rescale) {
-    for (int ch = half; ch * 32 < D; ch += 2) {
-      uint32_t r[32];
-      tmem_ld32(o_t + ch * 32, r);
-      tmem_wait_ld32(r);
+// O of this half's columns, times a factor per row.
+__device__ __forceinline__ void scale_o(uint32_t o_t, int D, int half, float factor) {
+#pragma unroll 1
+  for (int ch = half; ch * 32 < D; ch += 2) {
+    uint32_t r[32];
+    tmem_ld32(o_t + ch * 32, r);
+    tmem_wait_ld32(r);
 #pragma unroll
-      for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
-      tmem_st32(o_t + ch * 32, r);
+    for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
+    tmem_st32(o_t + ch * 32, r);
+  }
+}
+template <bool CAP, bool F16>
+__device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int half, float c, float cap_in, float cap_out, float ref,
+                                       float l, float sum, uint32_t sum_slot, uint32_t mx_slot, uint32_t word_mine, uint32_t stamp, bool valid,
+                                       bool stored, bool rescale, int left, volatile int *abort_flag) {
+  auto logits = [&](int ch, uint32_t (&r)[16]) {
+    tmem_ld16(s_t + ch * 16, r);
+    tmem_wait_ld16(r);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      float x = __uint_as_float(r[e]);
+      if (CAP) x = tanhf(x * cap_in) * cap_out;
+      r[e] = __float_as_uint(ch * 16 + e >= left ? -INFINITY : x * c);
+    }
+  };
+  // how far this half is above the reference: its maximum, or what its sum says of it
+  float mx = -INFINITY;
+  if (stored) {
+    mx = ref + log2f(sum);
+  } else {
+#pragma unroll 1
+    for (int ch = 0; ch < 4; ch++) {
+      uint32_t r[16];
+      logits(ch, r);
+#pragma unroll
+      for (int e = 0; e < 16; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
     }
   }
-  float sum = 0.f;
+  // (the slot of the tile before: both warps have read it)
+  asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(mx_slot), "f"(mx) : "memory");
+  redo_meet(word_mine, word_mine ^ 16, stamp, abort_flag);
+  float theirs;
+  asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(theirs) : "r"(mx_slot ^ 512) : "memory");
+  const float to = fmaxf(ref, fmaxf(mx, theirs));
+  float factor = 1.f;
+  if (valid && to > ref) {
+    factor = fast_exp2(ref - to);
+    ref = to;
+  }
+  if (rescale) scale_o(o_t, D, half, factor);
   if (stored) {
     uint32_t r[32];
     tmem_ld32(s_t, r);
@@ -297,20 +325,16 @@ __device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int ha
     for (int e = 0; e < 32; e++)
       r[e] = pack2<F16>(elem_value<F16>(r[e] & 0xffffu) * factor, elem_value<F16>(r[e] >> 16) * factor);
     tmem_st32(s_t, r);
+    sum *= factor;
   } else {
-    const float mc = m_used == -INFINITY ? 0.f : m_used * c;
+    sum = 0.f;
 #pragma unroll 1
     for (int ch = 0; ch < 4; ch++) {
-      uint32_t r[16];
-      tmem_ld16(s_t + ch * 16, r);
-      tmem_wait_ld16(r);
-      uint32_t t[8];
+      uint32_t r[16], t[8];
+      logits(ch, r);
 #pragma unroll
       for (int e = 0; e < 16; e++) {
-        float x = __uint_as_float(r[e]);
-        if (CAP) x = tanhf(x * cap_in) * cap_out;
-        if (ch * 16 + e >= left) x = -INFINITY;
-        const float pe = fast_exp2(fmaf(x, c, -mc));
+        const float pe = fast_exp2(__uint_as_float(r[e]) - ref);
         sum += pe;
         r[e] = __float_as_uint(pe);
       }
@@ -322,9 +346,29 @@ __device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int ha
   }
   tmem_wait_st();
   tc_fence_before();
-  redo_meet(word_mine, word_other, stamp + 1, abort_flag);
+  asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(sum_slot), "f"(sum) : "memory");
+  redo_meet(word_mine, word_mine ^ 16, stamp + 1, abort_flag);
   tc_fence_after();
-  return Redo{m_used, l * factor, sum};
+  return Redo{ref, l * factor, sum};
+}
+
+__device__ __forceinline__ uint64_t pair64(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpair64(uint64_t v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 template <int NBOX, bool CAP, bool F16>
@@ -494,21 +538,21 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     const uint32_t s_t = tmem + lane_base + i * 128 + half * 64;
     const uint32_t o_t = tmem + lane_base + 256 + i * 128;
     const int sync_id = 1 + i * 4 + quad;  // the two warps that share these rows
+    // this thread's word of the exchange; the other half's is 512 bytes on or back (the area is aligned)
     const uint32_t mine = smem_u32(xch) + ((i * 2 + half) * 128 + row) * 4;
-    const uint32_t theirs = mine + (half ? -512 : 512);
     constexpr uint32_t kSlot = Z::QT * 2 * 128 * 4;
-    const uint32_t word_mine = smem_u32(words + warp), word_other = smem_u32(words + (warp ^ 4));
-    uint32_t cnt = 0;  // logit tiles seen; the maxima of tile n are in slot n & 1
+    const uint32_t word_mine = smem_u32(words + warp);  // the other warp's: ^ 16
+    uint32_t cnt = 0;  // logit tiles seen; the sums of tile n are in slot n & 1
     const float c = p.scale * kLog2e;
     // soft-capping: x -> tanh(x*scale/cap)*cap/scale, so that x*c is the capped logit
     const float cap_in = p.scale / p.softcap, cap_out = p.softcap / p.scale;
-    // Probabilities of up to 2^kFar against the stale maximum are taken as they are: f16 ends at 2^16,
-    // bf16 and the fp32 sums have room for any that this leaves.
-    constexpr float kFar = F16 ? 15.f : 40.f;
+    // Sums of up to this much against the stale reference are taken as they are: f16 ends at 2^16, bf16
+    // and the fp32 accumulators have room for any that this leaves.
+    constexpr float kFar = F16 ? 32768.f : 1.099511627776e12f;
     auto put = [&](uint32_t slot, float x) { asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(mine + slot * kSlot), "f"(x) : "memory"); };
     auto get = [&](uint32_t slot) {
       float y;
-      asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(y) : "r"(theirs + slot * kSlot) : "memory");
+      asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(y) : "r"((mine ^ 512) + slot * kSlot) : "memory");
       return y;
     };
     // Waits for a barrier that cannot complete before both warps of these rows have announced tile
@@ -519,7 +563,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       bool met = false;
       while (!__all_sync(0xffffffffu, mbar_try_wait(b, parity))) {
         uint32_t w;
-        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(w) : "r"(word_other) : "memory");
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(w) : "r"(word_mine ^ 16) : "memory");
         if (!met && __any_sync(0xffffffffu, w == 2 * cnt)) {
           join();
           met = true;
@@ -543,16 +587,17 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       int min_lim = lim;
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, o));
-      float m_used = -INFINITY, l = 0.f, mx = -INFINITY;
-      bool behind = false;  // tile cnt - 1 belongs to this item and its meeting, if any, may be ahead
+      float ref = 0.f, l = 0.f, sum = 0.f;  // ref: 0 while the row has seen nothing
+      bool behind = false;  // tile cnt - 1 is this item's, and the other warp may yet call a meeting about it
       int left = 0;         // columns of the tile from here on are masked
       auto redo = [&](bool stored, bool rescale) {
         const uint32_t tile = stored ? cnt - 1 : cnt;
-        const Redo r = redo_tile<CAP, F16>(s_t, o_t, D, half, c, cap_in, cap_out, m_used, l, mx, theirs + (tile & 1) * kSlot, word_mine,
-                                           word_other, 2 * (tile + 1), valid, stored, rescale, left, abort_flag);
-        m_used = r.m_used;
+        const Redo r = redo_tile<CAP, F16>(s_t, o_t, D, half, c, cap_in, cap_out, ref, l, sum, mine + (tile & 1) * kSlot,
+                                           mine + (~tile & 1) * kSlot, word_mine, 2 * (tile + 1), valid, stored, rescale, left,
+                                           abort_flag);
+        ref = r.ref;
+        sum = r.sum;
         l = r.l;
-        return r.sum;
       };
       for (int t = g.kt0; t < g.kt1; t++, cnt++) {
         const bool first = t == g.kt0;
@@ -560,7 +605,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
           __syncwarp();
         } else {
-          wait_pending(bar(Z::B_SFULL + i), cnt & 1, [&] { behind ? (void)redo(true, t > g.kt0 + 1) : (void)0; });
+          wait_pending(bar(Z::B_SFULL + i), cnt & 1, [&] {
+            if (behind) redo(true, t > g.kt0 + 1);
+          });
         }
         tc_fence_after();
         const int key0 = t * kKeyTile + half * 64;
@@ -578,7 +625,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           }
         };
         if (first) {  // the first tile sets the reference
-          mx = -INFINITY;
+          float mx = -INFINITY;
 #pragma unroll 1
           for (int ch = 0; ch < 4; ch++) {
             uint32_t r[16];
@@ -590,71 +637,54 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           }
           put(cnt & 1, mx);
           pair_sync(sync_id);
-          m_used = fmaxf(mx, get(cnt & 1));
-          pair_sync(sync_id);  // both have read: the tile's own maxima go to the same place below
+          mx = fmaxf(mx, get(cnt & 1));
+          pair_sync(sync_id);  // both have read: the tile's own sums go to the same place below
+          ref = mx == -INFINITY ? 0.f : mx * c;
         } else {
-          // both halves of a row see the same maximum of the tile before and decide alike
-          mx = fmaxf(mx, get((cnt - 1) & 1));
-          const bool grew = valid && mx > m_used && !((mx - m_used) * c <= 8.f);
-          if (__any_sync(0xffffffffu, grew)) {
+          // both halves of a row see the same sum of the tile before and decide alike
+          const float both = sum + get((cnt - 1) & 1);
+          if (__any_sync(0xffffffffu, valid && both > 256.f)) {
             float factor = 1.f;
-            if (grew) {
-              factor = m_used == -INFINITY ? 0.f : fast_exp2((m_used - mx) * c);
-              m_used = mx;
+            if (valid && both > 256.f) {
+              factor = 1.f / both;
+              ref += log2f(both);
             }
             // O holds the tiles before this one: S of this tile was issued after their P.V
-#pragma unroll 1
-            for (int ch = half; ch * 32 < D; ch += 2) {
-              uint32_t r[32];
-              tmem_ld32(o_t + ch * 32, r);
-              tmem_wait_ld32(r);
-#pragma unroll
-              for (int e = 0; e < 32; e++) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
-              tmem_st32(o_t + ch * 32, r);
-            }
+            scale_o(o_t, D, half, factor);
             l *= factor;
           }
         }
-        float sum;
         uint32_t pr[32];  // the row half's probabilities, packed
         {
-          const float mc = m_used == -INFINITY ? 0.f : m_used * c;
-          float mxa[2] = {-INFINITY, -INFINITY}, sma[4] = {0.f, 0.f, 0.f, 0.f};
-          // 16 columns at a time, the next 16 on their way from TMEM meanwhile
-          uint32_t a[16], b[16];
-          auto part_pass = [&](uint32_t (&r)[16], int ch) {
+          const uint64_t c2 = pair64(c, c), ref2 = pair64(-ref, -ref);
+          uint64_t acc0 = 0, acc1 = 0;
+          // 16 columns at a time: a load takes some forty cycles, which the scheduler's other warps fill
+#pragma unroll
+          for (int ch = 0; ch < 4; ch++) {
+            uint32_t r[16];
+            tmem_ld16(s_t + ch * 16, r);
+            tmem_wait_ld16(r);
             cap_and_mask(r, ch * 16);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              const float x0 = __uint_as_float(r[e]), x1 = __uint_as_float(r[e + 1]);
-              mxa[(e >> 1) & 1] = fmaxf(mxa[(e >> 1) & 1], fmaxf(x0, x1));
-              const float p0 = fast_exp2(fmaf(x0, c, -mc)), p1 = fast_exp2(fmaf(x1, c, -mc));
-              sma[e & 2] += p0;
-              sma[(e & 2) + 1] += p1;
+              float x0, x1;
+              unpair64(fma2(pair64(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, ref2), x0, x1);
+              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              if (e & 2) acc1 = add2(acc1, pair64(p0, p1));
+              else acc0 = add2(acc0, pair64(p0, p1));
               pr[ch * 8 + (e >> 1)] = pack2<F16>(p0, p1);
             }
-          };
-          tmem_ld16(s_t, a);
-          tmem_wait_ld16(a);
-          tmem_ld16(s_t + 16, b);
-          part_pass(a, 0);
-          tmem_wait_ld16(b);
-          tmem_ld16(s_t + 32, a);
-          part_pass(b, 1);
-          tmem_wait_ld16(a);
-          tmem_ld16(s_t + 48, b);
-          part_pass(a, 2);
-          tmem_wait_ld16(b);
-          part_pass(b, 3);
-          mx = fmaxf(mxa[0], mxa[1]);
-          sum = (sma[0] + sma[1]) + (sma[2] + sma[3]);
+          }
+          float x0, x1;
+          unpair64(add2(acc0, acc1), x0, x1);
+          sum = x0 + x1;
         }
-        put(cnt & 1, mx);
         behind = true;
-        if (__any_sync(0xffffffffu, valid && (mx - m_used) * c > kFar)) {
-          sum = redo(false, !first);
+        if (__any_sync(0xffffffffu, valid && sum > kFar)) {
+          redo(false, !first);
           behind = false;
         } else {
+          put(cnt & 1, sum);
           tmem_st32(s_t, pr);
           tmem_wait_st();
           tc_fence_before();
@@ -672,9 +702,11 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             for (int e = ch * 32; e < D && e < ch * 32 + 32; e += 8) *reinterpret_cast<uint4 *>(orow + e) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] { behind ? (void)redo(true, g.kt1 > g.kt0 + 1) : (void)0; });
+      wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] {
+        if (behind) redo(true, g.kt1 > g.kt0 + 1);
+      });
       tc_fence_after();
-      pair_sync(sync_id);  // both are through with the maxima
+      pair_sync(sync_id);  // both are through with the last tile's sums
       put(0, l);
       pair_sync(sync_id);
       {
@@ -711,7 +743,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         __syncwarp();
       }
       if (!whole && valid && half == 0) {
-        part[(size_t)D * kRows] = m_used == -INFINITY ? -INFINITY : m_used * c;
+        part[(size_t)D * kRows] = l == 0.f ? -INFINITY : ref;  // a row that sees no key of this piece
         part[(size_t)(D + 1) * kRows] = l;
       }
       tc_fence_before();

@@ -598,6 +598,25 @@ def test_attend_logit_ranges(cuda_device, softcap, qk):
     r.check()
 
 
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("head", [64, 128, 192])
+@pytest.mark.parametrize("spikes", [[70], [130], [200], [130, 255], [140, 200, 300, 390], [511], [383, 640, 1022]])
+def test_attend_sudden_maxima(cuda_device, f16, head, spikes):
+    """Keys whose logits lie tens of powers of two above everything before them, in either half of a
+    key tile or in both, in the first, a middle and the last tile, for some rows and not for others."""
+    for q, kv in (([60], [1024]), ([300], [300]), ([700, 33], [1024, 1024])):
+        r = Attend(q, kv, 8, 2, head, f16=f16, seed=sum(spikes), qk=0.7)
+        sign = torch.where(torch.rand(r.q.shape[:2], generator=gen(5), device="cuda") < 0.6, 8.0, -8.0)
+        r.q[..., 0] = sign.to(r.q.dtype)
+        r.k[..., 0] = 0
+        for n, j in enumerate(spikes):
+            for base in r.cu_kv[:-1]:
+                if base + j < int(r.cu_kv[-1]):
+                    r.k[base + j, :, 0] = (60.0 + 40.0 * n) * head ** 0.5 / 8
+        r.run()
+        r.check()
+
+
 def test_attend_strides(cuda_device):
     r = Attend([33, 200], [133, 300], 8, 2, 96, seed=8, pad=3, first=2)
     r.run()
