@@ -266,10 +266,14 @@ __device__ __forceinline__ void redo_meet(uint32_t mine, uint32_t other, uint32_
   __threadfence_block();
   __syncwarp();
 }
+// 32-column chunks of O: the first half of them is one thread's of a row, the rest the other's.
+__device__ __forceinline__ int chunk_begin(int D, int half) { return half ? (((D + 31) >> 5) + 1) >> 1 : 0; }
+__device__ __forceinline__ int chunk_end(int D, int half) { return half ? (D + 31) >> 5 : (((D + 31) >> 5) + 1) >> 1; }
+
 // O of this half's columns, times a factor per row.
 __device__ __forceinline__ void scale_o(uint32_t o_t, int D, int half, float factor) {
 #pragma unroll 1
-  for (int ch = half; ch * 32 < D; ch += 2) {
+  for (int ch = chunk_begin(D, half); ch < chunk_end(D, half); ch++) {
     uint32_t r[32];
     tmem_ld32(o_t + ch * 32, r);
     tmem_wait_ld32(r);
@@ -391,6 +395,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G = p.G, D = p.D;
+  // the launch that joins partial results may be set up; it waits for this grid's end itself
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     mbar_init(bar(Z::B_QFULL), 1);
     mbar_init(bar(Z::B_QEMPTY), 1);
@@ -698,8 +704,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       elem16 *orow = p.out + q_row * p.out_stride + (int64_t)(g.h * G + head_in) * D;
       if (g.n == 0) {  // no key for any row of the item
         if (valid)
-          for (int ch = half; ch * 32 < D; ch += 2)
-            for (int e = ch * 32; e < D && e < ch * 32 + 32; e += 8) *reinterpret_cast<uint4 *>(orow + e) = make_uint4(0, 0, 0, 0);
+          for (int e = chunk_begin(D, half) * 32; e < min(chunk_end(D, half) * 32, D); e += 8)
+            *reinterpret_cast<uint4 *>(orow + e) = make_uint4(0, 0, 0, 0);
         continue;
       }
       wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] {
@@ -718,29 +724,63 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       constexpr int kRows = 128 * Z::QT;
       float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 2) * kRows + i * 128 + row;
       bool finite = true;
-      for (int ch = half; ch * 32 < D; ch += 2) {
-        uint32_t r[32];
-        tmem_ld32(o_t + ch * 32, r);
-        tmem_wait_ld32(r);
-        if (valid && whole) {
+      const int c0 = chunk_begin(D, half), c1 = chunk_end(D, half);
+      if (whole) {
+        // A thread has 64 bytes of its own row per chunk; four threads trade 16-byte pieces so that a
+        // store covers 64 bytes of eight rows instead of 16 bytes of thirty-two (a row apiece cost
+        // 4096 cycles of line accesses per item).
+        elem16 *row_at[4];
+        bool row_ok[4];
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float y[8];
+        for (int k = 0; k < 4; k++) {
+          const int src = (lane & ~3) + k;
+          row_at[k] = reinterpret_cast<elem16 *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), src)) + (lane & 3) * 8;
+          row_ok[k] = __shfl_sync(0xffffffffu, valid, src);
+        }
+        for (int ch = c0; ch < c1; ch++) {
+          uint32_t r[32];
+          tmem_ld32(o_t + ch * 32, r);
+          tmem_wait_ld32(r);
+          uint32_t w[4][4];  // piece, word
 #pragma unroll
-            for (int k = 0; k < 8; k++) y[k] = __uint_as_float(r[e + k]) * inv;
-            if (ch * 32 + e < D) {
+          for (int e = 0; e < 32; e += 2) {
+            const float y0 = __uint_as_float(r[e]) * inv, y1 = __uint_as_float(r[e + 1]) * inv;
+            if (ch * 32 + e < D) finite &= fabsf(y0) < INFINITY && fabsf(y1) < INFINITY;
+            w[e >> 3][(e >> 1) & 3] = pack2<F16>(y0, y1);
+          }
+          // 4 x 4 transpose of pieces over four lanes: piece b of lane a to piece a of lane b
 #pragma unroll
-              for (int k = 0; k < 8; k++) finite &= fabsf(y[k]) < INFINITY;
-              *reinterpret_cast<uint4 *>(orow + ch * 32 + e) =
-                  make_uint4(pack2<F16>(y[0], y[1]), pack2<F16>(y[2], y[3]), pack2<F16>(y[4], y[5]), pack2<F16>(y[6], y[7]));
+          for (int bit = 1; bit <= 2; bit <<= 1) {
+            const bool up = lane & bit;
+#pragma unroll
+            for (int a = 0; a < 4; a++) {
+              if (a & bit) continue;
+#pragma unroll
+              for (int k = 0; k < 4; k++) {
+                const uint32_t give = up ? w[a][k] : w[a | bit][k];
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, give, bit);
+                if (up) w[a][k] = got;
+                else w[a | bit][k] = got;
+              }
             }
           }
-        } else if (valid) {
 #pragma unroll
-          for (int e = 0; e < 32; e++)
-            if (ch * 32 + e < D) part[(size_t)(ch * 32 + e) * kRows] = __uint_as_float(r[e]);
+          for (int k = 0; k < 4; k++)
+            if (row_ok[k] && ch * 32 + (lane & 3) * 8 < D)
+              *reinterpret_cast<uint4 *>(row_at[k] + ch * 32) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
         }
-        __syncwarp();
+      } else {
+        for (int ch = c0; ch < c1; ch++) {
+          uint32_t r[32];
+          tmem_ld32(o_t + ch * 32, r);
+          tmem_wait_ld32(r);
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if (ch * 32 + e < D) part[(ch * 32 + e) * kRows] = __uint_as_float(r[e]);
+          }
+          __syncwarp();
+        }
       }
       if (!whole && valid && half == 0) {
         part[(size_t)D * kRows] = l == 0.f ? -INFINITY : ref;  // a row that sees no key of this piece
@@ -753,7 +793,11 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         const int src = __ffs(odd) - 1;
         odd &= odd - 1;
         const int tk = __shfl_sync(0xffffffffu, token, src), hd = g.h * G + __shfl_sync(0xffffffffu, head_in, src);
-        if (masked_value_not_finite(p, g.s, tk, g.h, g.n, F16)) repair_row<F16>(p, g.s, tk, hd, half ? 0xF0F0F0F0u : 0x0F0F0F0Fu);
+        if (masked_value_not_finite(p, g.s, tk, g.h, g.n, F16)) {
+          // pieces of eight columns, four to a chunk
+          const uint32_t below = (uint32_t)((1ull << (c0 * 4)) - 1), upto = (uint32_t)((1ull << (c1 * 4)) - 1);
+          repair_row<F16>(p, g.s, tk, hd, upto & ~below);
+        }
       }
     }
   }
@@ -785,10 +829,13 @@ struct JoinLaunch {
 };
 
 // Joins the partial results of the items that were cut: out = sum_c w_c O_c / sum_c w_c l_c with
-// w_c = 2^(m_c - max m), pieces in CTA order.  A warp takes 32 rows and 8 dimensions at a time;
-// partials are stored dimension-major, so that its loads are whole lines.
+// w_c = 2^(m_c - max m), pieces in CTA order.  A CTA takes 32 rows of an item: its warps fetch the
+// pieces' maxima and sums side by side, the weights go to shared memory, and then a warp takes
+// 8 dimensions of the rows at a time, the loads of four pieces in flight.  Partials are stored
+// dimension-major, so that loads are whole lines.  Bound by latency: launch, sums, rows.
 template <bool F16>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ JoinLaunch J) {
+  __shared__ float m_s[kMaxPlanCtas][32], l_s[kMaxPlanCtas][32];
   const PromptParams &p = J.p;
   const PlanPos it = J.item[blockIdx.x];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.D, G = p.G;
@@ -797,29 +844,44 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   const int q_len = p.cu_q[it.seq + 1] - p.cu_q[it.seq], kv_len = p.cu_kv[it.seq + 1] - p.cu_kv[it.seq];
   const int q0 = it.qt * J.tile_tokens, token = q0 + tile_i * J.sub_tokens + tok_in;
   const bool valid = tok_in < J.sub_tokens && token < q_len;
-  if (!__any_sync(0xffffffffu, valid)) return;
+  if (!__any_sync(0xffffffffu, valid)) return;  // the same rows in every warp
   const int n = (max(kv_len - q_len + min(q_len, q0 + J.tile_tokens), 0) + kKeyTile - 1) / kKeyTile;
-  const int c0 = J.first[blockIdx.x], c1 = J.last[blockIdx.x];
+  const int first = J.first[blockIdx.x], pieces = J.last[blockIdx.x] - first + 1;
   const size_t slot = (size_t)(D + 2) * J.rows;
   // the first piece begins the item: the second slot of its CTA; the others the first
-  auto part = [&](int c) { return J.ws + (size_t)(2 * c + (c == c0 ? 1 : 0)) * slot + row; };
+  const float *const at = J.ws + (size_t)(2 * first) * slot + row;
+  auto part = [&](int c) { return at + (size_t)(c == 0 ? 1 : 2 * c) * slot; };
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the attention kernel is through
+#pragma unroll 4
+  for (int c = warp; c < pieces; c += 8) {
+    m_s[c][lane] = valid ? part(c)[(size_t)D * J.rows] : -INFINITY;
+    l_s[c][lane] = valid ? part(c)[(size_t)(D + 1) * J.rows] : 0.f;
+  }
+  __syncthreads();
   float mx = -INFINITY, l = 0.f;
-  for (int c = c0; c <= c1; c++)
-    if (valid) mx = fmaxf(mx, part(c)[(size_t)D * J.rows]);
+  for (int c = 0; c < pieces; c++) mx = fmaxf(mx, m_s[c][lane]);
   const float base = mx == -INFINITY ? 0.f : mx;
-  for (int c = c0; c <= c1; c++)
-    if (valid) l += fast_exp2(part(c)[(size_t)D * J.rows] - base) * part(c)[(size_t)(D + 1) * J.rows];
+  for (int c = 0; c < pieces; c++) l += fast_exp2(m_s[c][lane] - base) * l_s[c][lane];
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   elem16 *orow = p.out + (int64_t)(p.cu_q[it.seq] + token) * p.out_stride + (int64_t)(it.head * G + head_in) * D;
   for (int d = warp * 8; d < D; d += 64) {
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int c = c0; c <= c1; c++) {
-      if (!valid) continue;
-      const float m = part(c)[(size_t)D * J.rows];
-      if (m == -INFINITY) continue;  // the row sees no key of this piece
-      const float wgt = fast_exp2(m - base);
+    for (int c = 0; c < pieces; c += 4) {
+      float x[4][8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) o[k] = fmaf(wgt, part(c)[(size_t)(d + k) * J.rows], o[k]);
+      for (int k = 0; k < 4; k++) {
+        // a row that sees no key of a piece has nothing there to add
+        const bool have = c + k < pieces && m_s[min(c + k, pieces - 1)][lane] != -INFINITY;
+        const float *src = part(c + k) + (size_t)d * J.rows;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[k][e] = have ? src[(size_t)e * J.rows] : 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const float wgt = fast_exp2(m_s[min(c + k, pieces - 1)][lane] - base);
+#pragma unroll
+        for (int e = 0; e < 8; e++) o[e] = fmaf(wgt, x[k][e], o[e]);
+      }
     }
     bool finite = true;
 #pragma unroll
@@ -949,10 +1011,19 @@ cudaError_t launch_prompt_attention(const PromptParams &p, bool f16, int num_sms
     most = std::max(most, left > shape.sub_tokens ? J.rows : std::min(left, shape.sub_tokens) * p.G);
   }
   const dim3 grid((unsigned)plan.num_split, (unsigned)(most + 31) / 32);
-  if (f16) prompt_join_kernel<true><<<grid, 256, 0, st>>>(J);
-  else prompt_join_kernel<false><<<grid, 256, 0, st>>>(J);
+  // a dependent launch: its CTAs are set up as the attention's retire
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = f16 ? cudaLaunchKernelEx(&cfg, prompt_join_kernel<true>, J) : cudaLaunchKernelEx(&cfg, prompt_join_kernel<false>, J);
   __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace pa
