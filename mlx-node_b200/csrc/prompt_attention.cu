@@ -46,6 +46,8 @@
 // copies in flight are drained and TMEM is freed.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "prompt_path.cuh"
 #include "tile_common.cuh"
 
@@ -159,11 +161,29 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 
-// V tile as the B operand of P.V, N (head dimension) contiguous: 128-byte swizzle, slabs of 64
-// dimensions kBox apart (leading byte offset), groups of 8 tokens 1024 B apart (stride).
-__device__ __forceinline__ uint64_t v_mn_desc(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(kBox >> 4) << 16) | (64ull << 32) | (1ull << 46) |
-         (2ull << 61);
+// Shared-memory matrix descriptors, 128-byte swizzle (layout 2, version 1).  The low word holds the
+// address and the leading byte offset, both in units of 16 bytes, so that a step along an operand is
+// an addition to it.  Q and K: K-major, groups of 8 rows 1024 B apart.  A V tile as the B operand of
+// P.V: MN-major (the head dimension contiguous), slabs of 64 dimensions kBox apart, groups of 8 tokens
+// 1024 B apart.
+constexpr uint32_t kDescHigh = 64u | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t k_major_low(uint32_t smem_addr) { return ((smem_addr >> 4) & 0x3FFFu) | (1u << 16); }
+__device__ __forceinline__ uint32_t mn_major_low(uint32_t smem_addr) {
+  return ((smem_addr >> 4) & 0x3FFFu) | ((uint32_t)(kBox >> 4) << 16);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %3};\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n}\n" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(kDescHigh), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_low, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b64 b;\n mov.b64 b, {%2, %3};\n setp.ne.b32 p, %5, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n}\n" ::"r"(d),
+      "r"(a_tmem), "r"(b_low), "r"(kDescHigh), "r"(idesc), "r"(acc)
+      : "memory");
 }
 // fp32 accumulator, M = 128; bit 16: B is MN-major
 __device__ __forceinline__ uint32_t mma_desc(bool f16, uint32_t n, bool b_mn) {
@@ -469,22 +489,19 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
 #pragma unroll
       for (int i = 0; i < Z::QT; i++) cnt[i] = 0;
       auto issue_s = [&](int i, uint32_t t) {
-        const uint32_t kst = k_s + (t % Z::NK) * Z::kTile;
+        const uint32_t a = k_major_low(q_s + i * Z::kTile), b = k_major_low(k_s + (t % Z::NK) * Z::kTile), d = tmem + i * 128;
 #pragma unroll
         for (int kk = 0; kk < NBOX * 4; kk++) {
-          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32;
-          if (leader && kk < ksteps)
-            umma_ss(tmem + i * 128, sw128_desc(q_s + i * Z::kTile + off), sw128_desc(kst + off), idesc_s, kk > 0 ? 1u : 0u);
+          const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
+          if (leader && kk < ksteps) mma_ss(d, a + off, b + off, idesc_s, kk > 0 ? 1u : 0u);
         }
         if (leader) tc_commit(bar(Z::B_SFULL + i));
       };
-      auto issue_pv = [&](int i, uint32_t t, bool first) {
-        const uint32_t vst = v_s + (t % Z::NV) * Z::kTile;
+      auto issue_pv = [&](int i, uint32_t t, uint32_t acc) {
+        const uint32_t b = mn_major_low(v_s + (t % Z::NV) * Z::kTile), a = tmem + i * 128, d = tmem + 256 + i * 128;
 #pragma unroll
         for (int kk = 0; kk < 8; kk++)
-          if (leader)
-            umma_ts(tmem + 256 + i * 128, tmem + i * 128 + (kk >> 2) * 64 + (kk & 3) * 8, v_mn_desc(vst + kk * 2048), idesc_pv,
-                    first && kk == 0 ? 0u : 1u);
+          if (leader) mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * 128, idesc_pv, kk > 0 ? 1u : acc);
         if (leader) tc_commit(bar(Z::B_PVDONE + i));
       };
       // S_i of key tile t into its buffer, once P_i.V of the tile before it is through with it
@@ -495,11 +512,12 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         cnt[i]++;
         return true;
       };
+      auto k_full = [&](uint32_t t) { return wait_all(bar(Z::B_KFULL + t % Z::NK), (t / Z::NK) & 1); };
+      auto v_full = [&](uint32_t t) { return wait_all(bar(Z::B_VFULL + t % Z::NV), (t / Z::NV) & 1); };
       while (!failed && walk_next<true>(L, at, g)) {
         const int n = g.kt1 - g.kt0;
         if (n <= 0) continue;
-        if (!wait_all(bar(Z::B_QFULL), items & 1) ||
-            !wait_all(bar(Z::B_KFULL + tiles % Z::NK), (tiles / Z::NK) & 1)) { failed = true; break; }
+        if (!wait_all(bar(Z::B_QFULL), items & 1) || !k_full(tiles)) { failed = true; break; }
 #pragma unroll
         for (int i = 0; i < Z::QT; i++)
           if (i < g.tiles && !failed) failed = !next_s(i, tiles);
@@ -510,17 +528,18 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         }
         for (int j = 0; j < n && !failed; j++) {
           const uint32_t t = tiles + j;
-          if (!wait_all(bar(Z::B_VFULL + t % Z::NV), (t / Z::NV) & 1)) { failed = true; break; }
+          const bool more = j + 1 < n;
+          // waited for while the softmax has the tile, not between its announcement and P.V
+          if (!v_full(t) || (more && !k_full(t + 1))) { failed = true; break; }
 #pragma unroll
           for (int i = 0; i < Z::QT; i++) {
             if (i >= g.tiles || failed) continue;
             if (!wait_all(bar(Z::B_PREADY + i), (cnt[i] - 1) & 1)) { failed = true; continue; }
             tc_fence_after();
-            issue_pv(i, t, j == 0);
+            issue_pv(i, t, j > 0 ? 1u : 0u);
             const bool last = i + 1 == g.tiles;
             if (last && leader) tc_commit(bar(Z::B_VEMPTY + t % Z::NV));
-            if (j + 1 < n) {
-              if (i == 0 && !wait_all(bar(Z::B_KFULL + (t + 1) % Z::NK), ((t + 1) / Z::NK) & 1)) { failed = true; continue; }
+            if (more) {
               if (!next_s(i, t + 1)) { failed = true; continue; }
               if (last && leader) {
                 tc_commit(bar(Z::B_KEMPTY + (t + 1) % Z::NK));
@@ -619,12 +638,12 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         const int key0 = t * kKeyTile + half * 64;
         const bool need_mask = key0 + 64 > min_lim;
         left = lim - key0;
-        auto cap_and_mask = [&](uint32_t (&r)[16], int col0) {
+        auto cap_and_mask = [&](uint32_t (&r)[16], int col0, bool mask) {
           if (CAP) {
 #pragma unroll
             for (int e = 0; e < 16; e++) r[e] = __float_as_uint(tanhf(__uint_as_float(r[e]) * cap_in) * cap_out);
           }
-          if (need_mask) {
+          if (mask) {
 #pragma unroll
             for (int e = 0; e < 16; e++)
               if (col0 + e >= left) r[e] = 0xff800000u;
@@ -637,7 +656,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             uint32_t r[16];
             tmem_ld16(s_t + ch * 16, r);
             tmem_wait_ld16(r);
-            cap_and_mask(r, ch * 16);
+            cap_and_mask(r, ch * 16, need_mask);
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
           }
@@ -661,7 +680,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           }
         }
         uint32_t pr[32];  // the row half's probabilities, packed
-        {
+        auto pass = [&](auto masked) {
+          constexpr bool MASK = decltype(masked)::value;
           const uint64_t c2 = pair64(c, c), ref2 = pair64(-ref, -ref);
           uint64_t acc0 = 0, acc1 = 0;
           // 16 columns at a time: a load takes some forty cycles, which the scheduler's other warps fill
@@ -670,12 +690,14 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             uint32_t r[16];
             tmem_ld16(s_t + ch * 16, r);
             tmem_wait_ld16(r);
-            cap_and_mask(r, ch * 16);
+            cap_and_mask(r, ch * 16, MASK);
 #pragma unroll
             for (int e = 0; e < 16; e += 2) {
-              float x0, x1;
-              unpair64(fma2(pair64(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, ref2), x0, x1);
-              const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+              const uint64_t x = fma2(pair64(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), c2, ref2);
+              float p0, p1;
+              unpair64(x, p0, p1);
+              p0 = fast_exp2(p0);
+              p1 = fast_exp2(p1);
               if (e & 2) acc1 = add2(acc1, pair64(p0, p1));
               else acc0 = add2(acc0, pair64(p0, p1));
               pr[ch * 8 + (e >> 1)] = pack2<F16>(p0, p1);
@@ -684,7 +706,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           float x0, x1;
           unpair64(add2(acc0, acc1), x0, x1);
           sum = x0 + x1;
-        }
+        };
+        if (need_mask) pass(std::true_type{});
+        else pass(std::false_type{});
         behind = true;
         if (__any_sync(0xffffffffu, valid && sum > kFar)) {
           redo(false, !first);
