@@ -761,6 +761,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           row_at[k] = reinterpret_cast<elem16 *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), src)) + (lane & 3) * 8;
           row_ok[k] = __shfl_sync(0xffffffffu, valid, src);
         }
+        const uint64_t inv2 = pair64(inv, inv);
+        uint64_t odd2 = 0;
         for (int ch = c0; ch < c1; ch++) {
           uint32_t r[32];
           tmem_ld32(o_t + ch * 32, r);
@@ -768,8 +770,12 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           uint32_t w[4][4];  // piece, word
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float y0 = __uint_as_float(r[e]) * inv, y1 = __uint_as_float(r[e + 1]) * inv;
-            if (ch * 32 + e < D) finite &= fabsf(y0) < INFINITY && fabsf(y1) < INFINITY;
+            const uint64_t y = fma2(pair64(__uint_as_float(r[e]), __uint_as_float(r[e + 1])), inv2, 0);
+            // 0 unless something is infinite or NaN (columns beyond D hold what an earlier item left: not
+            // looked at)
+            if (ch * 32 + e < D) odd2 = fma2(y, 0, odd2);
+            float y0, y1;
+            unpair64(y, y0, y1);
             w[e >> 3][(e >> 1) & 3] = pack2<F16>(y0, y1);
           }
           // 4 x 4 transpose of pieces over four lanes: piece b of lane a to piece a of lane b
@@ -793,6 +799,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             if (row_ok[k] && ch * 32 + (lane & 3) * 8 < D)
               *reinterpret_cast<uint4 *>(row_at[k] + ch * 32) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
         }
+        float odd0, odd1;
+        unpair64(odd2, odd0, odd1);
+        finite = odd0 == 0.f && odd1 == 0.f;
       } else {
         for (int ch = c0; ch < c1; ch++) {
           uint32_t r[32];
