@@ -15,7 +15,10 @@
 // Work: an item is up to 256 rows of one (sequence, kv head), a row being a (query token, head
 // of the group) pair, so that every key tile is read once for the whole group: two 128-row
 // query tiles that share each 128-key tile (head sizes above 128: one query tile, the
-// accumulator takes all the columns two would).  The line of items is cut into one piece of
+// accumulator takes all the columns two would).  An item of one query tile - single tokens, drafts,
+// the end of a prompt - gives the second tile's place to every other key tile: two accumulators with
+// references of their own, added at the end, so that the tensor cores and the softmax overlap there
+// too.  The line of items is cut into one piece of
 // equal cost per CTA (plan_prompt); an item that a cut splits leaves fp32 partial results in
 // the workspace, joined in CTA order by prompt_join_kernel, so that few rows over long keys
 // use every SM and the same call gives the same bits.
@@ -488,8 +491,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       uint32_t cnt[Z::QT];  // logit tiles issued for each query tile
 #pragma unroll
       for (int i = 0; i < Z::QT; i++) cnt[i] = 0;
-      auto issue_s = [&](int i, uint32_t t) {
-        const uint32_t a = k_major_low(q_s + i * Z::kTile), b = k_major_low(k_s + (t % Z::NK) * Z::kTile), d = tmem + i * 128;
+      auto issue_s = [&](int i, int q, uint32_t t) {
+        const uint32_t a = k_major_low(q_s + q * Z::kTile), b = k_major_low(k_s + (t % Z::NK) * Z::kTile), d = tmem + i * 128;
 #pragma unroll
         for (int kk = 0; kk < NBOX * 4; kk++) {
           const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32) >> 4;
@@ -504,11 +507,11 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           if (leader) mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * 128, idesc_pv, kk > 0 ? 1u : acc);
         if (leader) tc_commit(bar(Z::B_PVDONE + i));
       };
-      // S_i of key tile t into its buffer, once P_i.V of the tile before it is through with it
-      auto next_s = [&](int i, uint32_t t) {
+      // S_i = Q_q . K(t) into its buffer, once P_i.V of the tile before it is through with it
+      auto next_s = [&](int i, int q, uint32_t t) {
         if (cnt[i] > 0 && !wait_all(bar(Z::B_PVDONE + i), (cnt[i] - 1) & 1)) return false;
         tc_fence_after();
-        issue_s(i, t);
+        issue_s(i, q, t);
         cnt[i]++;
         return true;
       };
@@ -518,9 +521,42 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         const int n = g.kt1 - g.kt0;
         if (n <= 0) continue;
         if (!wait_all(bar(Z::B_QFULL), items & 1) || !k_full(tiles)) { failed = true; break; }
+        if constexpr (Z::QT == 2) if (g.tiles == 1) {
+          // one query tile: key tile j in place j % 2
+          failed = !next_s(0, 0, tiles);
+          if (!failed && leader) tc_commit(bar(Z::B_KEMPTY + tiles % Z::NK));
+          if (!failed && n > 1) {
+            failed = !k_full(tiles + 1) || !next_s(1, 0, tiles + 1);
+            if (!failed && leader) tc_commit(bar(Z::B_KEMPTY + (tiles + 1) % Z::NK));
+          }
+          if (!failed && n <= 2 && leader) tc_commit(bar(Z::B_QEMPTY));
+          for (int j0 = 0; j0 < n && !failed; j0 += 2) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int j = j0 + i;
+              const uint32_t t = tiles + j;
+              if (j >= n || failed) continue;
+              if (!v_full(t) || !wait_all(bar(Z::B_PREADY + i), (cnt[i] - 1) & 1)) { failed = true; continue; }
+              tc_fence_after();
+              issue_pv(i, t, j > 1 ? 1u : 0u);
+              if (leader) tc_commit(bar(Z::B_VEMPTY + t % Z::NV));
+              if (j + 2 < n) {
+                if (!k_full(t + 2) || !next_s(i, 0, t + 2)) { failed = true; continue; }
+                if (leader) {
+                  tc_commit(bar(Z::B_KEMPTY + (t + 2) % Z::NK));
+                  if (j + 3 == n) tc_commit(bar(Z::B_QEMPTY));
+                }
+              }
+            }
+            __syncwarp();
+          }
+          tiles += n;
+          items++;
+          continue;
+        }
 #pragma unroll
         for (int i = 0; i < Z::QT; i++)
-          if (i < g.tiles && !failed) failed = !next_s(i, tiles);
+          if (i < g.tiles && !failed) failed = !next_s(i, i, tiles);
         if (failed) break;
         if (leader) {
           tc_commit(bar(Z::B_KEMPTY + tiles % Z::NK));
@@ -540,7 +576,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             const bool last = i + 1 == g.tiles;
             if (last && leader) tc_commit(bar(Z::B_VEMPTY + t % Z::NV));
             if (more) {
-              if (!next_s(i, t + 1)) { failed = true; continue; }
+              if (!next_s(i, i, t + 1)) { failed = true; continue; }
               if (last && leader) {
                 tc_commit(bar(Z::B_KEMPTY + (t + 1) % Z::NK));
                 if (j + 2 == n) tc_commit(bar(Z::B_QEMPTY));
@@ -605,8 +641,11 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     // returns at once): two of them share each row's barrier, and one that left would leave
     // the other waiting at it.
     while (walk_next<true>(L, at, g)) {
-      if (i >= g.tiles) continue;
-      const int token = g.q0 + i * L.sub_tokens + tok_in;  // within the sequence
+      // one query tile, two places: this one takes every other key tile from `start` on
+      const bool both_places = Z::QT == 2 && g.tiles == 1;
+      const int step = both_places ? 2 : 1, start = g.kt0 + (both_places ? i : 0);
+      if (i >= g.tiles && !(both_places && start < g.kt1)) continue;
+      const int token = g.q0 + (both_places ? 0 : i * L.sub_tokens) + tok_in;  // within the sequence
       const bool valid = tok_in < L.sub_tokens && token < g.q_len;
       const int lim = valid ? g.kv_len - g.q_len + token + 1 : 0x7fffffff;  // keys the row sees
       int min_lim = lim;
@@ -624,14 +663,14 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         sum = r.sum;
         l = r.l;
       };
-      for (int t = g.kt0; t < g.kt1; t++, cnt++) {
-        const bool first = t == g.kt0;
+      for (int t = start; t < g.kt1; t += step, cnt++) {
+        const bool first = t == start;
         if (first) {
           failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
           __syncwarp();
         } else {
           wait_pending(bar(Z::B_SFULL + i), cnt & 1, [&] {
-            if (behind) redo(true, t > g.kt0 + 1);
+            if (behind) redo(true, t > start + step);
           });
         }
         tc_fence_after();
@@ -733,7 +772,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         continue;
       }
       wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] {
-        if (behind) redo(true, g.kt1 > g.kt0 + 1);
+        if (behind) redo(true, g.kt1 > start + step);
       });
       tc_fence_after();
       pair_sync(sync_id);  // both are through with the last tile's sums
@@ -744,6 +783,46 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         l = half == 0 ? l + l_other : l_other + l;
       }
       pair_sync(sync_id);
+      if (both_places && g.kt0 + 1 < g.kt1) {
+        // place 1 hands its reference and sum to place 0, which reads both accumulators
+        auto quad_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(9 + quad) : "memory"); };
+        if (i == 1) {
+          put(0, l == 0.f ? -INFINITY : ref);
+          put(1, l);
+          tc_fence_before();
+          quad_sync();
+          quad_sync();  // O_1 has been read
+          continue;
+        }
+        quad_sync();
+        tc_fence_after();
+        float ref1, l1;
+        asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(ref1) : "r"(mine + 1024) : "memory");
+        asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(l1) : "r"(mine + 1024 + kSlot) : "memory");
+        // a place whose keys the row does not see counts for nothing (its P was 0, its P.V may be NaN)
+        const float top = fmaxf(l == 0.f ? -INFINITY : ref, ref1);
+        const float f0 = l == 0.f ? 0.f : fast_exp2(ref - top);  // O = f0 O_0 + f1 O_1
+        const float f1 = l1 == 0.f ? 0.f : fast_exp2(ref1 - top);
+        l = f0 * l + f1 * l1;
+        if (top != -INFINITY) ref = top;
+#pragma unroll 1
+        for (int ch = chunk_begin(D, half); ch < chunk_end(D, half); ch++) {
+          uint32_t r[32], r1[32];
+          tmem_ld32(o_t + ch * 32, r);
+          tmem_ld32(o_t + 128 + ch * 32, r1);
+          tmem_wait_ld32(r);
+          tmem_wait_ld32(r1);
+#pragma unroll
+          for (int e = 0; e < 32; e++) {
+            const float a = f0 == 0.f ? 0.f : f0 * __uint_as_float(r[e]), b = f1 == 0.f ? 0.f : f1 * __uint_as_float(r1[e]);
+            r[e] = __float_as_uint(a + b);
+          }
+          tmem_st32(o_t + ch * 32, r);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        quad_sync();
+      }
       const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
       constexpr int kRows = 128 * Z::QT;
       float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 2) * kRows + i * 128 + row;

@@ -240,7 +240,7 @@ struct PromptPlan {
 // Costs in sixteenths of the time of a key tile with two query tiles.
 constexpr int kMinPiece = 2;         // a piece of an item is at least this many key tiles
 constexpr int kMinTilesPerCta = 3;   // and a CTA gets work worth this many
-constexpr int kCostTwo = 16, kCostOne = 11, kCostItem = 20, kCostZero = 4;
+constexpr int kCostTwo = 16, kCostOne = 9, kCostItem = 31, kCostZero = 4;
 
 // Plans sequences [s0, s1) of the batch (at most kMaxPlanSeqs).
 inline void plan_prompt(const int32_t *cu_q, const int32_t *cu_kv, int32_t s0, int32_t s1, int32_t num_kv_heads,
