@@ -73,7 +73,7 @@ struct Geo {
   static constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK,
                        B_VEMPTY = B_VFULL + NV, B_SFULL = B_VEMPTY + NV, B_PREADY = B_SFULL + QT,
                        B_PVDONE = B_PREADY + QT, kBars = B_PVDONE + QT;
-  static constexpr int kXch = 2 * QT * 2 * 128 * 4;     // [parity][query tile][half][row] floats
+  static constexpr int kXch = 4 * QT * 2 * 128 * 4;     // [slot][query tile][half][row] floats
   static constexpr int kWalk = kThreads / 32 * 16;       // a PlanPos per warp
   static constexpr int kWords = 8 * QT * 4;             // a meeting word per softmax warp
   static constexpr int kSmem = 1024 + (QT + NK + NV) * kTile + kXch + kWalk + kWords + kBars * 8 + 16;
@@ -307,7 +307,7 @@ __device__ __forceinline__ void scale_o(uint32_t o_t, int D, int half, float fac
 }
 template <bool CAP, bool F16>
 __device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int half, float c, float cap_in, float cap_out, float ref,
-                                       float l, float sum, uint32_t sum_slot, uint32_t mx_slot, uint32_t word_mine, uint32_t stamp, bool valid,
+                                       float l, float sum, uint32_t sum_slot, uint32_t mx_slot, uint32_t l_slot, uint32_t word_mine, uint32_t stamp, bool valid,
                                        bool stored, bool rescale, int left, volatile int *abort_flag) {
   auto logits = [&](int ch, uint32_t (&r)[16]) {
     tmem_ld16(s_t + ch * 16, r);
@@ -374,6 +374,7 @@ __device__ __noinline__ Redo redo_tile(uint32_t s_t, uint32_t o_t, int D, int ha
   tmem_wait_st();
   tc_fence_before();
   asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(sum_slot), "f"(sum) : "memory");
+  if (stored) asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(l_slot), "f"(l * factor) : "memory");
   redo_meet(word_mine, word_mine ^ 16, stamp + 1, abort_flag);
   tc_fence_after();
   return Redo{ref, l * factor, sum};
@@ -442,6 +443,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;
+  // set up while the kernel ahead was finishing; what it wrote is read, and what it read written, from
+  // here on only
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   bool failed = false;
   Seg g;
   if (lane == 0) *at = L.begin[blockIdx.x];
@@ -603,7 +607,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     const uint32_t mine = smem_u32(xch) + ((i * 2 + half) * 128 + row) * 4;
     constexpr uint32_t kSlot = Z::QT * 2 * 128 * 4;
     const uint32_t word_mine = smem_u32(words + warp);  // the other warp's: ^ 16
-    uint32_t cnt = 0;  // logit tiles seen; the sums of tile n are in slot n & 1
+    // slots 0 and 1: the sums of even and odd tiles; slot 2: an item's sum;
+    // slot 3: the maxima of an item's first tile
+    uint32_t cnt = 0;  // logit tiles seen
     const float c = p.scale * kLog2e;
     // soft-capping: x -> tanh(x*scale/cap)*cap/scale, so that x*c is the capped logit
     const float cap_in = p.scale / p.softcap, cap_out = p.softcap / p.scale;
@@ -657,7 +663,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       auto redo = [&](bool stored, bool rescale) {
         const uint32_t tile = stored ? cnt - 1 : cnt;
         const Redo r = redo_tile<CAP, F16>(s_t, o_t, D, half, c, cap_in, cap_out, ref, l, sum, mine + (tile & 1) * kSlot,
-                                           mine + (~tile & 1) * kSlot, word_mine, 2 * (tile + 1), valid, stored, rescale, left,
+                                           mine + (~tile & 1) * kSlot, mine + 2 * kSlot, word_mine, 2 * (tile + 1), valid, stored, rescale, left,
                                            abort_flag);
         ref = r.ref;
         sum = r.sum;
@@ -699,10 +705,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
 #pragma unroll
             for (int e = 0; e < 16; e++) mx = fmaxf(mx, __uint_as_float(r[e]));
           }
-          put(cnt & 1, mx);
+          put(3, mx);
           pair_sync(sync_id);
-          mx = fmaxf(mx, get(cnt & 1));
-          pair_sync(sync_id);  // both have read: the tile's own sums go to the same place below
+          mx = fmaxf(mx, get(3));
           ref = mx == -INFINITY ? 0.f : mx * c;
         } else {
           // both halves of a row see the same sum of the tile before and decide alike
@@ -759,6 +764,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           tc_fence_before();
         }
         l += sum;
+        if (t + step >= g.kt1) put(2, l);  // read after P.V of this tile, for which both warps have arrived
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(Z::B_PREADY + i));
       }
@@ -775,14 +781,10 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         if (behind) redo(true, g.kt1 > start + step);
       });
       tc_fence_after();
-      pair_sync(sync_id);  // both are through with the last tile's sums
-      put(0, l);
-      pair_sync(sync_id);
       {
-        const float l_other = get(0);
+        const float l_other = get(2);
         l = half == 0 ? l + l_other : l_other + l;
       }
-      pair_sync(sync_id);
       if (both_places && g.kt0 + 1 < g.kt1) {
         // place 1 hands its reference and sum to place 0, which reads both accumulators
         auto quad_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(9 + quad) : "memory"); };
@@ -1032,17 +1034,34 @@ bool encode_rows(CUtensorMap *map, const void *ptr, int D, int heads, int64_t ro
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A launch whose CTAs may be set up before the kernel ahead on the stream has finished.
+template <typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, int threads, int smem, cudaStream_t st, const Args &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int NBOX>
 cudaError_t launch_boxes(const PromptLaunch &L, const CUtensorMap &qm, const CUtensorMap &km, const CUtensorMap &vm,
                          bool f16, int ctas, cudaStream_t st) {
   const bool cap = L.p.softcap != 1.0f;
-  auto go = [&](auto kernel) { kernel<<<ctas, Geo<NBOX>::kThreads, Geo<NBOX>::kSmem, st>>>(L, qm, km, vm); };
+  cudaError_t e = cudaSuccess;
+  auto go = [&](auto kernel) { e = launch_dependent(kernel, dim3(ctas), Geo<NBOX>::kThreads, Geo<NBOX>::kSmem, st, L, qm, km, vm); };
   if (cap && f16) go(prompt_attention_kernel<NBOX, true, true>);
   else if (cap) go(prompt_attention_kernel<NBOX, true, false>);
   else if (f16) go(prompt_attention_kernel<NBOX, false, true>);
   else go(prompt_attention_kernel<NBOX, false, false>);
-  __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace
@@ -1123,19 +1142,8 @@ cudaError_t launch_prompt_attention(const PromptParams &p, bool f16, int num_sms
     most = std::max(most, left > shape.sub_tokens ? J.rows : std::min(left, shape.sub_tokens) * p.G);
   }
   const dim3 grid((unsigned)plan.num_split, (unsigned)(most + 31) / 32);
-  // a dependent launch: its CTAs are set up as the attention's retire
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  e = f16 ? cudaLaunchKernelEx(&cfg, prompt_join_kernel<true>, J) : cudaLaunchKernelEx(&cfg, prompt_join_kernel<false>, J);
-  __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
-  return e;
+  return f16 ? launch_dependent(prompt_join_kernel<true>, grid, 256, 0, st, J)
+             : launch_dependent(prompt_join_kernel<false>, grid, 256, 0, st, J);
 }
 
 }  // namespace pa

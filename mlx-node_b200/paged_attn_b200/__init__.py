@@ -190,14 +190,18 @@ def _check(status: int) -> None:
 
 
 def _ptr(x) -> int:
+    # in the order of how often a call passes them: a call's own time on the host is a few
+    # microseconds, of which a numpy array's .ctypes alone would be one
     if x is None:
         return 0
+    data_ptr = getattr(x, "data_ptr", None)
+    if data_ptr is not None:
+        return data_ptr()
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
-    if hasattr(x, "ctypes"):  # numpy array (host memory)
-        return x.ctypes.data
+    array = getattr(x, "__array_interface__", None)  # numpy array (host memory)
+    if array is not None:
+        return array["data"][0]
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
