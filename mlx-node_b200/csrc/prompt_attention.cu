@@ -43,7 +43,8 @@
 //
 // A probability of a masked key is exactly 0, but 0 * NaN is NaN: a row whose result is not
 // finite is checked for masked values that are not, and then recomputed by itself over the keys
-// that it sees (repair_row).  The check costs a comparison per output element.
+// that it sees (repair_row).  So is a bf16 row that is not finite after a sum above 2^60 (a logit
+// 41 above everything in the tiles before).  The check costs a comparison per output element.
 //
 // Every wait is bounded; on expiry the CTA raises the error word, every role leaves its loop,
 // copies in flight are drained and TMEM is freed.
@@ -72,8 +73,8 @@ struct Geo {
   static constexpr int kThreads = (kSoft + 4) * 32;     // whole warpgroups
   static constexpr int B_QFULL = 0, B_QEMPTY = 1, B_KFULL = 2, B_KEMPTY = B_KFULL + NK, B_VFULL = B_KEMPTY + NK,
                        B_VEMPTY = B_VFULL + NV, B_SFULL = B_VEMPTY + NV, B_PREADY = B_SFULL + QT,
-                       B_PVDONE = B_PREADY + QT, kBars = B_PVDONE + QT;
-  static constexpr int kXch = 4 * QT * 2 * 128 * 4;     // [slot][query tile][half][row] floats
+                       B_PHALF = B_PREADY + QT, B_PVDONE = B_PHALF + QT, kBars = B_PVDONE + QT;
+  static constexpr int kXch = 5 * QT * 2 * 128 * 4;     // [slot][query tile][half][row] floats
   static constexpr int kWalk = kThreads / 32 * 16;       // a PlanPos per warp
   static constexpr int kWords = 8 * QT * 4;             // a meeting word per softmax warp
   static constexpr int kSmem = 1024 + (QT + NK + NV) * kTile + kXch + kWalk + kWords + kBars * 8 + 16;
@@ -83,7 +84,7 @@ struct Geo {
 struct PromptLaunch {
   PromptParams p;
   PlanPos begin[kMaxPlanCtas + 1];
-  float *ws;       // two partial slots per CTA, each [D + 2][128 * QT] floats
+  float *ws;       // two partial slots per CTA, each [D + 3][128 * QT] floats: O, reference, sum, far
   unsigned *err;
   int32_t sub_tokens, tile_tokens;
 };
@@ -265,8 +266,8 @@ __device__ __noinline__ bool masked_value_not_finite(const PromptParams &p, int 
   return __any_sync(0xffffffffu, bad);
 }
 
-// The rare case that a logit of the current tile is so far above the reference that its probability
-// would leave the 16-bit type's (f16) or the accumulator's comfortable range: the two warps of a set
+// f16: the rare case that a logit of the current tile is so far above the reference that its probability
+// would leave the type's range: the two warps of a set
 // of rows meet and settle on the tile's own maximum before the tile's P.V may start.  One of them
 // found the case before it stored its probabilities and takes them again from the logits; the other
 // may have stored and announced its own (`stored`) and scales those.  Neither can run ahead: P.V
@@ -429,6 +430,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     for (int i = 0; i < Z::QT; i++) {
       mbar_init(bar(Z::B_SFULL + i), 1);
       mbar_init(bar(Z::B_PREADY + i), 8);
+      mbar_init(bar(Z::B_PHALF + i), 8);
       mbar_init(bar(Z::B_PVDONE + i), 1);
     }
     for (int i = 0; i < 8 * Z::QT; i++) words[i] = 0;
@@ -504,12 +506,25 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         }
         if (leader) tc_commit(bar(Z::B_SFULL + i));
       };
+      // P_i.V(t), as the softmax announces it (the issuing warp waits): bf16 in two halves, the first
+      // while the second half's probabilities are still being taken
       auto issue_pv = [&](int i, uint32_t t, uint32_t acc) {
         const uint32_t b = mn_major_low(v_s + (t % Z::NV) * Z::kTile), a = tmem + i * 128, d = tmem + 256 + i * 128;
+        if (!F16) {
+          if (!wait_all(bar(Z::B_PHALF + i), (cnt[i] - 1) & 1)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; kk++)
+            if (leader && !(kk & 2)) mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * 128, idesc_pv, kk > 0 ? 1u : acc);
+        }
+        if (!wait_all(bar(Z::B_PREADY + i), (cnt[i] - 1) & 1)) return false;
+        tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < 8; kk++)
-          if (leader) mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * 128, idesc_pv, kk > 0 ? 1u : acc);
+          if (leader && (F16 || (kk & 2)))
+            mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b + kk * 128, idesc_pv, !F16 || kk > 0 ? 1u : acc);
         if (leader) tc_commit(bar(Z::B_PVDONE + i));
+        return true;
       };
       // S_i = Q_q . K(t) into its buffer, once P_i.V of the tile before it is through with it
       auto next_s = [&](int i, int q, uint32_t t) {
@@ -540,9 +555,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
               const int j = j0 + i;
               const uint32_t t = tiles + j;
               if (j >= n || failed) continue;
-              if (!v_full(t) || !wait_all(bar(Z::B_PREADY + i), (cnt[i] - 1) & 1)) { failed = true; continue; }
-              tc_fence_after();
-              issue_pv(i, t, j > 1 ? 1u : 0u);
+              if (!v_full(t) || !issue_pv(i, t, j > 1 ? 1u : 0u)) { failed = true; continue; }
               if (leader) tc_commit(bar(Z::B_VEMPTY + t % Z::NV));
               if (j + 2 < n) {
                 if (!k_full(t + 2) || !next_s(i, 0, t + 2)) { failed = true; continue; }
@@ -574,9 +587,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
 #pragma unroll
           for (int i = 0; i < Z::QT; i++) {
             if (i >= g.tiles || failed) continue;
-            if (!wait_all(bar(Z::B_PREADY + i), (cnt[i] - 1) & 1)) { failed = true; continue; }
-            tc_fence_after();
-            issue_pv(i, t, j > 0 ? 1u : 0u);
+            if (!issue_pv(i, t, j > 0 ? 1u : 0u)) { failed = true; continue; }
             const bool last = i + 1 == g.tiles;
             if (last && leader) tc_commit(bar(Z::B_VEMPTY + t % Z::NV));
             if (more) {
@@ -613,9 +624,10 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     const float c = p.scale * kLog2e;
     // soft-capping: x -> tanh(x*scale/cap)*cap/scale, so that x*c is the capped logit
     const float cap_in = p.scale / p.softcap, cap_out = p.softcap / p.scale;
-    // Sums of up to this much against the stale reference are taken as they are: f16 ends at 2^16, bf16
-    // and the fp32 accumulators have room for any that this leaves.
-    constexpr float kFar = F16 ? 32768.f : 1.099511627776e12f;
+    // Sums of up to this much against the stale reference are taken as they are.  f16 ends at 2^16; bf16 has
+    // fp32's range, and its probabilities are announced before the sum is known.
+    // (bf16: beyond this a row that comes out not finite is recomputed, see `far`)
+    constexpr float kFar = F16 ? 32768.f : 1.152921504606847e18f;
     auto put = [&](uint32_t slot, float x) { asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(mine + slot * kSlot), "f"(x) : "memory"); };
     auto get = [&](uint32_t slot) {
       float y;
@@ -660,7 +672,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       float ref = 0.f, l = 0.f, sum = 0.f;  // ref: 0 while the row has seen nothing
       bool behind = false;  // tile cnt - 1 is this item's, and the other warp may yet call a meeting about it
       int left = 0;         // columns of the tile from here on are masked
-      auto redo = [&](bool stored, bool rescale) {
+      bool far = false;     // bf16: a sum was so large that an overflow is this kernel's own
+      [[maybe_unused]] auto redo = [&](bool stored, bool rescale) {
         const uint32_t tile = stored ? cnt - 1 : cnt;
         const Redo r = redo_tile<CAP, F16>(s_t, o_t, D, half, c, cap_in, cap_out, ref, l, sum, mine + (tile & 1) * kSlot,
                                            mine + (~tile & 1) * kSlot, mine + 2 * kSlot, word_mine, 2 * (tile + 1), valid, stored, rescale, left,
@@ -671,7 +684,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       };
       for (int t = start; t < g.kt1; t += step, cnt++) {
         const bool first = t == start;
-        if (first) {
+        if (first || !F16) {
           failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
           __syncwarp();
         } else {
@@ -746,6 +759,13 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
               else acc0 = add2(acc0, pair64(p0, p1));
               pr[ch * 8 + (e >> 1)] = pack2<F16>(p0, p1);
             }
+            if (!F16 && ch == 1) tmem_st16(s_t, reinterpret_cast<uint32_t (&)[16]>(pr[0]));
+            if (!F16 && ch == 2) {  // the first half has been on its way for a quarter of the pass
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(Z::B_PHALF + i));
+            }
           }
           float x0, x1;
           unpair64(add2(acc0, acc1), x0, x1);
@@ -753,18 +773,29 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         };
         if (need_mask) pass(std::true_type{});
         else pass(std::false_type{});
-        behind = true;
-        if (__any_sync(0xffffffffu, valid && sum > kFar)) {
-          redo(false, !first);
-          behind = false;
+        if constexpr (F16) {
+          behind = true;
+          if (__any_sync(0xffffffffu, valid && sum > kFar)) {
+            redo(false, !first);
+            behind = false;
+          } else {
+            put(cnt & 1, sum);
+            tmem_st32(s_t, pr);
+            tmem_wait_st();
+            tc_fence_before();
+          }
         } else {
+          far |= sum > kFar;
+          tmem_st16(s_t + 16, reinterpret_cast<uint32_t (&)[16]>(pr[16]));
           put(cnt & 1, sum);
-          tmem_st32(s_t, pr);
           tmem_wait_st();
           tc_fence_before();
         }
         l += sum;
-        if (t + step >= g.kt1) put(2, l);  // read after P.V of this tile, for which both warps have arrived
+        if (t + step >= g.kt1) {  // read after P.V of this tile, for which both warps have arrived
+          put(2, l);
+          if (!F16) put(4, far ? 1.f : 0.f);
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(Z::B_PREADY + i));
       }
@@ -777,13 +808,19 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
             *reinterpret_cast<uint4 *>(orow + e) = make_uint4(0, 0, 0, 0);
         continue;
       }
-      wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] {
-        if (behind) redo(true, g.kt1 > start + step);
-      });
+      if (F16) {
+        wait_pending(bar(Z::B_PVDONE + i), (cnt - 1) & 1, [&] {
+          if (behind) redo(true, g.kt1 > start + step);
+        });
+      } else {
+        failed |= !wait_bar(bar(Z::B_PVDONE + i), (cnt - 1) & 1, abort_flag);
+        __syncwarp();
+      }
       tc_fence_after();
       {
         const float l_other = get(2);
         l = half == 0 ? l + l_other : l_other + l;
+        if (!F16) far |= get(4) != 0.f;
       }
       if (both_places && g.kt0 + 1 < g.kt1) {
         // place 1 hands its reference and sum to place 0, which reads both accumulators
@@ -791,6 +828,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         if (i == 1) {
           put(0, l == 0.f ? -INFINITY : ref);
           put(1, l);
+          if (!F16) put(3, far ? 1.f : 0.f);
           tc_fence_before();
           quad_sync();
           quad_sync();  // O_1 has been read
@@ -801,6 +839,11 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         float ref1, l1;
         asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(ref1) : "r"(mine + 1024) : "memory");
         asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(l1) : "r"(mine + 1024 + kSlot) : "memory");
+        if (!F16) {
+          float far1;
+          asm volatile("ld.volatile.shared.f32 %0, [%1];" : "=f"(far1) : "r"(mine + 1024 + 3 * kSlot) : "memory");
+          far |= far1 != 0.f;
+        }
         // a place whose keys the row does not see counts for nothing (its P was 0, its P.V may be NaN)
         const float top = fmaxf(l == 0.f ? -INFINITY : ref, ref1);
         const float f0 = l == 0.f ? 0.f : fast_exp2(ref - top);  // O = f0 O_0 + f1 O_1
@@ -827,7 +870,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       }
       const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
       constexpr int kRows = 128 * Z::QT;
-      float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 2) * kRows + i * 128 + row;
+      float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 3) * kRows + i * 128 + row;
       bool finite = true;
       const int c0 = chunk_begin(D, half), c1 = chunk_end(D, half);
       if (whole) {
@@ -899,6 +942,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       if (!whole && valid && half == 0) {
         part[(size_t)D * kRows] = l == 0.f ? -INFINITY : ref;  // a row that sees no key of this piece
         part[(size_t)(D + 1) * kRows] = l;
+        part[(size_t)(D + 2) * kRows] = far ? 1.f : 0.f;
       }
       tc_fence_before();
       uint32_t odd = __ballot_sync(0xffffffffu, valid && !finite);
@@ -907,7 +951,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         const int src = __ffs(odd) - 1;
         odd &= odd - 1;
         const int tk = __shfl_sync(0xffffffffu, token, src), hd = g.h * G + __shfl_sync(0xffffffffu, head_in, src);
-        if (masked_value_not_finite(p, g.s, tk, g.h, g.n, F16)) {
+        const bool own = __shfl_sync(0xffffffffu, far, src);  // the row overflowed here and not in its values
+        if (own || masked_value_not_finite(p, g.s, tk, g.h, g.n, F16)) {
           // pieces of eight columns, four to a chunk
           const uint32_t below = (uint32_t)((1ull << (c0 * 4)) - 1), upto = (uint32_t)((1ull << (c1 * 4)) - 1);
           repair_row<F16>(p, g.s, tk, hd, upto & ~below);
@@ -950,6 +995,7 @@ struct JoinLaunch {
 template <bool F16>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ JoinLaunch J) {
   __shared__ float m_s[kMaxPlanCtas][32], l_s[kMaxPlanCtas][32];
+  __shared__ int far_s[32];
   const PromptParams &p = J.p;
   const PlanPos it = J.item[blockIdx.x];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, D = p.D, G = p.G;
@@ -961,7 +1007,9 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   if (!__any_sync(0xffffffffu, valid)) return;  // the same rows in every warp
   const int n = (max(kv_len - q_len + min(q_len, q0 + J.tile_tokens), 0) + kKeyTile - 1) / kKeyTile;
   const int first = J.first[blockIdx.x], pieces = J.last[blockIdx.x] - first + 1;
-  const size_t slot = (size_t)(D + 2) * J.rows;
+  const size_t slot = (size_t)(D + 3) * J.rows;
+  if (warp == 0) far_s[lane] = 0;
+  __syncthreads();
   // the first piece begins the item: the second slot of its CTA; the others the first
   const float *const at = J.ws + (size_t)(2 * first) * slot + row;
   auto part = [&](int c) { return at + (size_t)(c == 0 ? 1 : 2 * c) * slot; };
@@ -970,6 +1018,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   for (int c = warp; c < pieces; c += 8) {
     m_s[c][lane] = valid ? part(c)[(size_t)D * J.rows] : -INFINITY;
     l_s[c][lane] = valid ? part(c)[(size_t)(D + 1) * J.rows] : 0.f;
+    if (valid && part(c)[(size_t)(D + 2) * J.rows] != 0.f) far_s[lane] = 1;
   }
   __syncthreads();
   float mx = -INFINITY, l = 0.f;
@@ -1012,7 +1061,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
       const int src = __ffs(odd) - 1;
       odd &= odd - 1;
       const int tk = __shfl_sync(0xffffffffu, token, src), hd = it.head * G + __shfl_sync(0xffffffffu, head_in, src);
-      if (masked_value_not_finite(p, it.seq, tk, it.head, n, F16)) repair_row<F16>(p, it.seq, tk, hd, 1u << (d >> 3));
+      if (far_s[src] || masked_value_not_finite(p, it.seq, tk, it.head, n, F16)) repair_row<F16>(p, it.seq, tk, hd, 1u << (d >> 3));
     }
   }
 }
@@ -1068,7 +1117,7 @@ cudaError_t launch_boxes(const PromptLaunch &L, const CUtensorMap &qm, const CUt
 
 size_t prompt_workspace_bytes(int num_sms, int head_size) {
   const size_t rows = head_size <= 128 ? 256 : 128;
-  return (size_t)2 * std::min(num_sms, kMaxPlanCtas) * rows * (head_size + 2) * 4;
+  return (size_t)2 * std::min(num_sms, kMaxPlanCtas) * rows * (head_size + 3) * 4;
 }
 
 cudaError_t prompt_configure() {
