@@ -994,7 +994,7 @@ struct JoinLaunch {
 // dimension-major, so that loads are whole lines.  Bound by latency: launch, sums, rows.
 template <bool F16>
 __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant__ JoinLaunch J) {
-  __shared__ float m_s[kMaxPlanCtas][32], l_s[kMaxPlanCtas][32];
+  extern __shared__ float join_smem[];  // the pieces' references, then their sums
   __shared__ int far_s[32];
   const PromptParams &p = J.p;
   const PlanPos it = J.item[blockIdx.x];
@@ -1007,6 +1007,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   if (!__any_sync(0xffffffffu, valid)) return;  // the same rows in every warp
   const int n = (max(kv_len - q_len + min(q_len, q0 + J.tile_tokens), 0) + kKeyTile - 1) / kKeyTile;
   const int first = J.first[blockIdx.x], pieces = J.last[blockIdx.x] - first + 1;
+  float(*const m_s)[32] = reinterpret_cast<float(*)[32]>(join_smem), (*const l_s)[32] = m_s + pieces;
   const size_t slot = (size_t)(D + 3) * J.rows;
   if (warp == 0) far_s[lane] = 0;
   __syncthreads();
@@ -1182,17 +1183,19 @@ cudaError_t launch_prompt_attention(const PromptParams &p, bool f16, int num_sms
   J.sub_tokens = shape.sub_tokens;
   J.tile_tokens = shape.tile_tokens;
   J.rows = shape.tile_tokens > shape.sub_tokens ? 256 : 128;
-  int most = 0;  // rows of the largest item that is cut
+  int most = 0, pieces = 0;  // rows of the largest item that is cut, pieces of the one cut most often
   for (int k = 0; k < plan.num_split; k++) {
     J.item[k] = plan.begin[plan.split_last[k]];
     J.first[k] = plan.split_first[k];
     J.last[k] = plan.split_last[k];
+    pieces = std::max(pieces, plan.split_last[k] - plan.split_first[k] + 1);
     const int left = p.cu_q[J.item[k].seq + 1] - p.cu_q[J.item[k].seq] - J.item[k].qt * shape.tile_tokens;
     most = std::max(most, left > shape.sub_tokens ? J.rows : std::min(left, shape.sub_tokens) * p.G);
   }
   const dim3 grid((unsigned)plan.num_split, (unsigned)(most + 31) / 32);
-  return f16 ? launch_dependent(prompt_join_kernel<true>, grid, 256, 0, st, J)
-             : launch_dependent(prompt_join_kernel<false>, grid, 256, 0, st, J);
+  const int smem = pieces * 2 * 32 * 4;  // 40 KB for an item over all CTAs
+  return f16 ? launch_dependent(prompt_join_kernel<true>, grid, 256, smem, st, J)
+             : launch_dependent(prompt_join_kernel<false>, grid, 256, smem, st, J);
 }
 
 }  // namespace pa

@@ -239,7 +239,7 @@ struct PromptPlan {
 
 // Costs in sixteenths of the time of a key tile with two query tiles.
 constexpr int kMinPiece = 2;         // a piece of an item is at least this many key tiles
-constexpr int kMinTilesPerCta = 3;   // and a CTA gets work worth this many
+constexpr int kMinTilesPerCta = 2;   // and a CTA gets work worth this many
 constexpr int kCostTwo = 16, kCostOne = 9, kCostItem = 31, kCostZero = 4;
 
 // Plans sequences [s0, s1) of the batch (at most kMaxPlanSeqs).
