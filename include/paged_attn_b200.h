@@ -289,8 +289,8 @@ pa_status pa_rope_frequencies(const PaRope *rope, double *frequencies, float *ga
  *   q_norm_weight, k_norm_weight  [head_size] in the cache dtype, or null for no norm
  *   positions    int32 [num_tokens], device; any value
  *   slot_mapping int64 [num_tokens], device, or null: nothing is written to the pool (v may
- *                then be null).  Skipping and reporting as in pa_reshape_and_cache; of two
- *                tokens with one slot either may be the one that stays
+ *                then be null).  Skipping and reporting as in pa_reshape_and_cache; no two
+ *                tokens may name one slot (what stays there is not defined)
  * The pool bytes after the call are those pa_reshape_and_cache would have written from
  * k_out and v (an FP8 cache quantises the 16-bit key with the layer's scales).     */
 pa_status pa_rope_norm_and_cache(PagedAttnCache *cache, uint32_t layer_idx, const PaRope *rope,

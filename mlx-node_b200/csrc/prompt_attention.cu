@@ -76,7 +76,7 @@ struct Geo {
                        B_PHALF = B_PREADY + QT, B_PVDONE = B_PHALF + QT, kBars = B_PVDONE + QT;
   static constexpr int kXch = 5 * QT * 2 * 128 * 4;     // [slot][query tile][half][row] floats
   static constexpr int kWalk = kThreads / 32 * 16;       // a PlanPos per warp
-  static constexpr int kWords = 8 * QT * 4;             // a meeting word per softmax warp
+  static constexpr int kWords = 8 * QT * 4 + 16;        // a meeting word per softmax warp, the beat
   static constexpr int kSmem = 1024 + (QT + NK + NV) * kTile + kXch + kWalk + kWords + kBars * 8 + 16;
   static_assert(kSmem <= 232448, "shared memory per CTA");
 };
@@ -192,6 +192,28 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_l
 // fp32 accumulator, M = 128; bit 16: B is MN-major
 __device__ __forceinline__ uint32_t mma_desc(bool f16, uint32_t n, bool b_mn) {
   return (1u << 4) | (f16 ? 0u : ((1u << 7) | (1u << 10))) | (b_mn ? 1u << 16 : 0u) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// wait_bar with a second chance: a softmax warp that recomputes rows by itself (repair_row) counts them
+// in `beat`, and the roles that wait for it meanwhile start their second anew with every count.
+__device__ __forceinline__ bool wait_live(uint32_t bar, uint32_t parity, volatile int *abort_flag, volatile uint32_t *beat) {
+  if (mbar_try_wait(bar, parity)) return true;
+  long long t0 = clock64();
+  uint32_t seen = *beat;
+  int spins = 0;
+  while (!mbar_try_wait(bar, parity)) {
+    if ((++spins & 63) == 0) {
+      if (*abort_flag) return false;
+      if (*beat != seen) {
+        seen = *beat;
+        t0 = clock64();
+      } else if (clock64() - t0 > (1ll << 31)) {
+        *abort_flag = 1;
+        return false;
+      }
+    }
+  }
+  return true;
 }
 
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
@@ -412,7 +434,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
   float *xch = reinterpret_cast<float *>(gen + (Z::QT + Z::NK + Z::NV) * Z::kTile);
   PlanPos *const at = reinterpret_cast<PlanPos *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch) + (threadIdx.x >> 5);
   uint32_t *const words = reinterpret_cast<uint32_t *>(reinterpret_cast<uint8_t *>(xch) + Z::kXch + Z::kWalk);
-  uint64_t *bars = reinterpret_cast<uint64_t *>(words + 8 * Z::QT);
+  volatile uint32_t *const beat = words + 8 * Z::QT;
+  uint64_t *bars = reinterpret_cast<uint64_t *>(words + 8 * Z::QT + 4);
   uint32_t *tmem_holder = reinterpret_cast<uint32_t *>(bars + Z::kBars);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_holder + 1);
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
@@ -433,7 +456,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       mbar_init(bar(Z::B_PHALF + i), 8);
       mbar_init(bar(Z::B_PVDONE + i), 1);
     }
-    for (int i = 0; i < 8 * Z::QT; i++) words[i] = 0;
+    for (int i = 0; i <= 8 * Z::QT; i++) words[i] = 0;
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -463,7 +486,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         uint32_t items = 0, tiles = 0;  // items and key tiles fetched so far
         while (!failed && walk_next<false>(L, at, g)) {
           if (g.kt0 >= g.kt1) continue;
-          if (items > 0 && !wait_bar(bar(Z::B_QEMPTY), (items - 1) & 1, abort_flag)) { failed = true; break; }
+          if (items > 0 && !wait_live(bar(Z::B_QEMPTY), (items - 1) & 1, abort_flag, beat)) { failed = true; break; }
           mbar_expect_tx(bar(Z::B_QFULL), (uint32_t)(g.tiles * NBOX * L.sub_tokens * G) * 128u);
           for (int i = 0; i < g.tiles; i++)
             for (int b = 0; b < NBOX; b++)
@@ -473,11 +496,11 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           for (int t = g.kt0; t < g.kt1; t++, tiles++) {
             const int row = p.cu_kv[g.s] + t * kKeyTile;
             const int ks = tiles % Z::NK, vs = tiles % Z::NV;
-            if (tiles >= Z::NK && !wait_bar(bar(Z::B_KEMPTY + ks), (tiles / Z::NK - 1) & 1, abort_flag)) { failed = true; break; }
+            if (tiles >= Z::NK && !wait_live(bar(Z::B_KEMPTY + ks), (tiles / Z::NK - 1) & 1, abort_flag, beat)) { failed = true; break; }
             mbar_expect_tx(bar(Z::B_KFULL + ks), Z::kTile);
             for (int b = 0; b < NBOX; b++)
               tma_load_3d(k_s + ks * Z::kTile + b * kBox, &k_map, b * 64, g.h, row, bar(Z::B_KFULL + ks));
-            if (tiles >= Z::NV && !wait_bar(bar(Z::B_VEMPTY + vs), (tiles / Z::NV - 1) & 1, abort_flag)) { failed = true; break; }
+            if (tiles >= Z::NV && !wait_live(bar(Z::B_VEMPTY + vs), (tiles / Z::NV - 1) & 1, abort_flag, beat)) { failed = true; break; }
             mbar_expect_tx(bar(Z::B_VFULL + vs), Z::kTile);
             for (int b = 0; b < NBOX; b++)
               tma_load_3d(v_s + vs * Z::kTile + b * kBox, &v_map, b * 64, g.h, row, bar(Z::B_VFULL + vs));
@@ -489,7 +512,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       // =========================== MMA issue ===========================================
       // The whole warp walks the loop so that descriptors and addresses stay warp-uniform; one
       // elected lane issues.  Its waits end alike for every lane.
-      auto wait_all = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(b, parity, abort_flag)) != 0; };
+      auto wait_all = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, wait_live(b, parity, abort_flag, beat)) != 0; };
       const uint32_t idesc_s = mma_desc(F16, 128, false), idesc_pv = mma_desc(F16, (uint32_t)(D + 15) & ~15u, true);
       const int ksteps = (D + 15) >> 4;
       const bool leader = elect_one();
@@ -638,7 +661,8 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     // cnt - 1; meanwhile the other one may call for a meeting about that tile (redo_tile).
     auto wait_pending = [&](uint32_t b, uint32_t parity, auto &&join) {
       if (__all_sync(0xffffffffu, mbar_try_wait(b, parity))) return;
-      const long long t0 = clock64();
+      long long t0 = clock64();
+      uint32_t seen = *beat;
       bool met = false;
       while (!__all_sync(0xffffffffu, mbar_try_wait(b, parity))) {
         uint32_t w;
@@ -648,6 +672,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           met = true;
         }
         if (*abort_flag) failed = true;
+        if (*beat != seen) seen = *beat, t0 = clock64();
         if (clock64() - t0 > (1ll << 31)) failed = true, *abort_flag = 1;
         if (__any_sync(0xffffffffu, failed)) {
           failed = true;
@@ -685,7 +710,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       for (int t = start; t < g.kt1; t += step, cnt++) {
         const bool first = t == start;
         if (first || !F16) {
-          failed |= !wait_bar(bar(Z::B_SFULL + i), cnt & 1, abort_flag);
+          failed |= !wait_live(bar(Z::B_SFULL + i), cnt & 1, abort_flag, beat);
           __syncwarp();
         } else {
           wait_pending(bar(Z::B_SFULL + i), cnt & 1, [&] {
@@ -813,7 +838,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           if (behind) redo(true, g.kt1 > start + step);
         });
       } else {
-        failed |= !wait_bar(bar(Z::B_PVDONE + i), (cnt - 1) & 1, abort_flag);
+        failed |= !wait_live(bar(Z::B_PVDONE + i), (cnt - 1) & 1, abort_flag, beat);
         __syncwarp();
       }
       tc_fence_after();
@@ -957,6 +982,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           const uint32_t below = (uint32_t)((1ull << (c0 * 4)) - 1), upto = (uint32_t)((1ull << (c1 * 4)) - 1);
           repair_row<F16>(p, g.s, tk, hd, upto & ~below);
         }
+        if (lane == 0) atomicAdd(const_cast<uint32_t *>(beat), 1u);
       }
     }
   }
@@ -1162,7 +1188,7 @@ cudaError_t launch_prompt_attention(const PromptParams &p, bool f16, int num_sms
   L.tile_tokens = shape.tile_tokens;
   CUtensorMap qm, km, vm;
   bool ok = encode_rows(&qm, p.q, p.D, p.Hq, p.cu_q[p.S], p.q_stride, p.G, shape.sub_tokens);
-  if (p.cu_kv[p.S] > 0) {
+  if (p.cu_kv[p.S] > p.cu_kv[0]) {
     ok = ok && encode_rows(&km, p.k, p.D, p.Hkv, p.cu_kv[p.S], p.k_stride, 1, kKeyTile) &&
          encode_rows(&vm, p.v, p.D, p.Hkv, p.cu_kv[p.S], p.v_stride, 1, kKeyTile);
   } else {

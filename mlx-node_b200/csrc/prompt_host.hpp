@@ -168,6 +168,9 @@ inline ArgError check_prompt_args(const PagedAttnConfig &cfg, const void *out, c
   if (!ptr16(out) || !ptr16(q) || !ptr16(k) || !ptr16(v)) return bad_arg("tensors must be 16-byte aligned");
   if (!(scale > 0.f) || !(softcap > 0.f) || !std::isfinite(scale) || !std::isfinite(softcap))
     return bad_arg("scale and softcap must be finite and > 0");
+  if (softcap != 1.0f && !std::isfinite(softcap / scale)) return bad_arg("softcap / scale must be finite");
+  if (cu_q[num_seqs] > INT32_MAX - 1024 || ckv[num_seqs] > INT32_MAX - 1024)
+    return bad_arg("more than 2^31 - 1024 query or key rows");
   if (!workspace || workspace_bytes < need_bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u))
     return bad_arg("workspace missing, too small or not 256-byte aligned");
   return {};

@@ -185,7 +185,12 @@ int main() {
     EXPECT(prompt(p, p, cu, cu, 4, 512, 1.f, -1.f, p, 1000) == PA_ERR_INVALID_ARG);
     EXPECT(prompt(p, p, cu, cu, 4, 512, 1.f, 1.f, p, 999) == PA_ERR_INVALID_ARG);
     EXPECT(prompt(p, p, cu, cu, 4, 512, 1.f, 1.f, odd, 1000) == PA_ERR_INVALID_ARG);
-    const int32_t none[] = {0, 0, 0};
+    EXPECT(prompt(p, p, cu, cu, 4, 512, 1e-38f, 30.f, p, 1000) == PA_ERR_INVALID_ARG);  // softcap / scale
+    const int32_t huge[] = {0, 5, INT32_MAX};
+    EXPECT(prompt(p, p, cu, huge, 4, 512, 1.f, 1.f, p, 1000) == PA_ERR_INVALID_ARG);
+    EXPECT(prompt(p, p, huge, huge, 4, 512, 1.f, 1.f, p, 1000) == PA_ERR_INVALID_ARG);
+    const int32_t none[] = {0, 0, 0}, later[] = {7, 7, 7};
+    EXPECT(prompt(p, nullptr, cu, later, 4, 512, 1.f, 1.f, p, 1000) == PA_OK);
     EXPECT(prompt(nullptr, nullptr, none, cu, 4, 512, 1.f, 1.f, nullptr, 0) == PA_OK);
     EXPECT(prompt(p, nullptr, cu, none, 4, 512, 1.f, 1.f, p, 1000) == PA_OK);
 

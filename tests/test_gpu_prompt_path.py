@@ -553,6 +553,8 @@ def test_attend_rows_without_keys(cuda_device):
         r.check()
         assert (r.out[4:4 + 130, :8] == 0).all() and (r.out[304:309, :8] == 0).all()
     r = Attend([4, 2], [0, 0], 4, 2, 128)
+    r.cu_kv += 11  # no key anywhere, and no buffer of keys
+    r.k, r.v = torch.empty(0, 2, 128, dtype=r.k.dtype, device="cuda"), torch.empty(0, 2, 128, dtype=r.k.dtype, device="cuda")
     r.run()
     torch.cuda.synchronize()
     assert (r.out[:6] == 0).all() and (r.out[6:] == 7.0).all()
@@ -601,9 +603,11 @@ def test_attend_logit_ranges(cuda_device, softcap, qk):
 @pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("head", [64, 128, 192])
 @pytest.mark.parametrize("spikes", [[70], [130], [200], [130, 255], [140, 200, 300, 390], [511], [383, 640, 1022]])
-def test_attend_sudden_maxima(cuda_device, f16, head, spikes):
-    """Keys whose logits lie tens of powers of two above everything before them, in either half of a
-    key tile or in both, in the first, a middle and the last tile, for some rows and not for others."""
+@pytest.mark.parametrize("height", [60.0, 160.0])
+def test_attend_sudden_maxima(cuda_device, f16, head, spikes, height):
+    """Keys whose logits lie tens of powers of two above everything before them - or more than fp32's
+    exponent - in either half of a key tile or in both, in the first, a middle and the last tile, for
+    some rows and not for others."""
     for q, kv in (([60], [1024]), ([300], [300]), ([700, 33], [1024, 1024])):
         r = Attend(q, kv, 8, 2, head, f16=f16, seed=sum(spikes), qk=0.7)
         sign = torch.where(torch.rand(r.q.shape[:2], generator=gen(5), device="cuda") < 0.6, 8.0, -8.0)
@@ -612,7 +616,7 @@ def test_attend_sudden_maxima(cuda_device, f16, head, spikes):
         for n, j in enumerate(spikes):
             for base in r.cu_kv[:-1]:
                 if base + j < int(r.cu_kv[-1]):
-                    r.k[base + j, :, 0] = (60.0 + 40.0 * n) * head ** 0.5 / 8
+                    r.k[base + j, :, 0] = (height + 40.0 * n) * head ** 0.5 / 8
         r.run()
         r.check()
 
@@ -656,6 +660,30 @@ def test_attend_masked_places_do_not_reach(cuda_device):
             same = (r.out[:rows] == clean[:rows]).flatten(1).all(1)
             assert same[:40].all(), "another sequence's values reached the first one"
             assert torch.isnan(r.out[rows:347]).any(-1).all(), "a row that sees a NaN key has to show it"
+
+
+@pytest.mark.parametrize("f16", [False, True])
+def test_attend_masked_places_of_a_cut_item(cuda_device, f16):
+    """The same where the item is cut over many CTAs and rows are put right by the join, and where it
+    is one query tile on two places."""
+    for q, kv, hq, hkv in ((3, 9000, 8, 1), (40, 6000, 4, 1), (100, 3000, 8, 2)):
+        r = Attend([q, 2], [kv, 50], hq, hkv, 128, seed=q, f16=f16)
+        r.run()
+        torch.cuda.synchronize()
+        clean = r.out.clone()
+        r.v[kv - 1, :, 3] = float("nan")   # the last query alone sees it
+        r.v[kv - 2] = float("inf")         # the last two
+        r.v[kv + 10:] = float("nan")       # the other sequence
+        r.run()
+        torch.cuda.synchronize()
+        r.cache.check_errors()
+        got = r.out[:q - 2]
+        ref, mag = attend_exact(r.q[:q - 2], r.k[:kv - 2], r.v[:kv - 2], [0, q - 2], [0, kv - 2], r.scale)
+        assert torch.isfinite(got).all() and ((got.double() - ref).abs() <= attend_bound(got.dtype, ref, mag, kv)).all()
+        assert (r.out[q - 2, :, :] == float("inf")).all() and torch.isnan(r.out[q - 1, :, 3]).all()
+        assert (r.out[q - 1, :, 4:] == float("inf")).all()
+        same = (got == clean[:q - 2]) | ((got.double() - clean[:q - 2].double()).abs() <= attend_bound(got.dtype, ref, mag, kv))
+        assert same.all()
 
 
 def test_attend_special_values_propagate(cuda_device):
