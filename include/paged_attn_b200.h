@@ -66,8 +66,9 @@ int32_t pa_version(void);
  * 16 - and, up to head size 120, with the reference's default block_size 32 -
  * dtype 0 or 1, no FP8 cache (KV write, decode and multi-token attention;
  * chunks of more than 24 / G query tokens - 16 / G with head size 192, 8 / G with
- * 256 - are served in pieces and need context_lens_host, the fused producer
- * launch is refused, pa_decode_step runs its two kernels).  dtype 2 returns
+ * 256 - are served in pieces and need context_lens_host, pa_qk_norm_rope_and_cache
+ * is refused (pa_rope_norm_and_cache takes every cache), pa_decode_step runs its two
+ * kernels).  dtype 2 returns
  * PA_ERR_UNSUPPORTED.  An FP8 cache needs block_size 16 or 32, as in the
  * reference (config.rs:71-76).                                                 */
 typedef struct PagedAttnConfig {

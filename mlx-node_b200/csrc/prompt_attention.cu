@@ -46,6 +46,11 @@
 // that it sees (repair_row).  So is a bf16 row that is not finite after a sum above 2^60 (a logit
 // 41 above everything in the tiles before).  The check costs a comparison per output element.
 //
+// Bound by the chain of one query tile (S - softmax - P.V - S), 3200 cycles per 128 keys of both
+// query tiles against 2350 of tensor pipe; measured on one B200: 8192-token prompt, 32/8 heads of
+// 128, bf16, 485-540 us (1.0-1.1 PFLOP/s); two chunks of 1024 over 4096 163-169 us; eight sequences
+// of 1-5 tokens over 4000-16000 keys 72-80 us (4.5-4.9 TB/s).
+//
 // Every wait is bounded; on expiry the CTA raises the error word, every role leaves its loop,
 // copies in flight are drained and TMEM is freed.
 #include <cuda.h>

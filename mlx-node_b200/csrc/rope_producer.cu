@@ -24,6 +24,8 @@
 // multiple of 8 elements: a shuffle) or, for the odd sizes, are read again from global memory.  The
 // value chunk is a transpose of the rows: where a CTA's 16 tokens fill an aligned run of slots it is
 // stored in runs of tokens out of ldmatrix.trans (FP8: byte permutes), otherwise element by element.
+// Measured on one B200: 8192 tokens, 32/8 heads of 128, keys kept, 218 MB in 50.9 us (4.3 TB/s); 2049
+// tokens, 64/8 heads, FP8 write, 84 MB in 24.9 us; one token 4.3 us in a graph.
 #include <algorithm>
 #include <type_traits>
 
