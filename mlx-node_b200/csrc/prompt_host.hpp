@@ -215,14 +215,23 @@ inline bool operator==(const PlanPos &a, const PlanPos &b) {
   return a.seq == b.seq && a.head == b.head && a.qt == b.qt && a.kt == b.kt;
 }
 
+constexpr int kMinPiece = 2;         // a piece of an item is at least this many key tiles
+constexpr int kMinTilesPerCta = 2;   // and a CTA gets work worth this many
+// Costs in sixteenths of the time of a key tile with two query tiles (fitted to the CTAs' own times:
+// an item costs two key tiles besides its tiles; one query tile alone runs two key tiles at a time,
+// except with head sizes above 128).
+constexpr int kCostTwo = 16, kCostOne = 9, kCostItem = 31, kCostZero = 4;
+
 struct PromptShape {
   int32_t tile_tokens;  // query tokens of an item: tiles * (128 / group)
   int32_t sub_tokens;   // query tokens of one 128-row tile
+  int32_t cost_one;     // of a key tile with one query tile
 };
 inline PromptShape prompt_shape(int head_size, int group) {
   PromptShape s;
   s.sub_tokens = kTileRows / group;
   s.tile_tokens = s.sub_tokens * (head_size <= 128 ? 2 : 1);
+  s.cost_one = head_size <= 128 ? kCostOne : kCostTwo;
   return s;
 }
 
@@ -239,11 +248,6 @@ struct PromptPlan {
   int32_t split_first[kMaxPlanCtas];  // first and last CTA of each item that is cut
   int32_t split_last[kMaxPlanCtas];
 };
-
-// Costs in sixteenths of the time of a key tile with two query tiles.
-constexpr int kMinPiece = 2;         // a piece of an item is at least this many key tiles
-constexpr int kMinTilesPerCta = 2;   // and a CTA gets work worth this many
-constexpr int kCostTwo = 16, kCostOne = 9, kCostItem = 31, kCostZero = 4;
 
 // Plans sequences [s0, s1) of the batch (at most kMaxPlanSeqs).
 inline void plan_prompt(const int32_t *cu_q, const int32_t *cu_kv, int32_t s0, int32_t s1, int32_t num_kv_heads,
@@ -263,7 +267,7 @@ inline void plan_prompt(const int32_t *cu_q, const int32_t *cu_kv, int32_t s0, i
       prefix.push_back(sum);
       const int32_t q1 = std::min(ql - q, shape.tile_tokens) + q;
       const int32_t n = plan_key_tiles(ql, kl, q1);
-      sum += n == 0 ? kCostZero : kCostItem + (int64_t)n * (q1 - q > shape.sub_tokens ? kCostTwo : kCostOne);
+      sum += n == 0 ? kCostZero : kCostItem + (int64_t)n * (q1 - q > shape.sub_tokens ? kCostTwo : shape.cost_one);
       q = q1;
     }
     prefix.push_back(sum);
@@ -303,7 +307,7 @@ inline void plan_prompt(const int32_t *cu_q, const int32_t *cu_kv, int32_t s0, i
     const int64_t q0 = (int64_t)p.qt * shape.tile_tokens;
     const int32_t q1 = (int32_t)std::min<int64_t>(q0 + shape.tile_tokens, ql);
     const int32_t kts = plan_key_tiles(ql, kl, q1);
-    const int32_t unit = q1 - q0 > shape.sub_tokens ? kCostTwo : kCostOne;
+    const int32_t unit = q1 - q0 > shape.sub_tokens ? kCostTwo : shape.cost_one;
     const int64_t kt = kts == 0 || r <= kCostItem / 2 ? 0 : std::max<int64_t>(0, (r - kCostItem + unit / 2) / unit);
     if (c > 0) {
       if (kt < min_piece) p.kt = 0;
