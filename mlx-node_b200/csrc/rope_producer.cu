@@ -25,7 +25,7 @@
 // value chunk is a transpose of the rows: where a CTA's 16 tokens fill an aligned run of slots it is
 // stored in runs of tokens out of ldmatrix.trans (FP8: byte permutes), otherwise element by element.
 // Measured on one B200: 8192 tokens, 32/8 heads of 128, keys kept, 218 MB in 50.9 us (4.3 TB/s); 2049
-// tokens, 64/8 heads, FP8 write, 84 MB in 24.9 us; one token 4.3 us in a graph.
+// tokens, 64/8 heads, FP8 write, 84 MB in 22.7 us; one token 4.3 us in a graph.
 #include <algorithm>
 #include <type_traits>
 
@@ -51,38 +51,66 @@ __device__ __forceinline__ void unpack8(uint4 v, float (&x)[8]) {
 __device__ __forceinline__ bool has_exponent15(uint2 b) {
   return ((((b.x & 0x78787878u) + 0x08080808u) | ((b.y & 0x78787878u) + 0x08080808u)) & 0x80808080u) != 0u;
 }
+__device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("min.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
 
-// quantise8 for the common case, bit for bit: eight elements whose scaled magnitudes are all in
-// [2^-6, 240) take the hardware's E4M3 conversion, which rounds that range to nearest even like the
-// cache format does; anything else - smaller, larger, infinity, NaN - goes to the format's own
-// encoder.  x / scale is rounded to fp32 as IEEE division does, by Markstein's correction
-// (IBM J. Res. Dev. 34, 1990): with y the correctly rounded reciprocal, q = x y and
-// q + (x - q scale) y is the correctly rounded quotient as long as nothing under- or overflows,
-// which `scale` in [2^-60, 2^60] and the range above make sure of.
+// quantise8 for the common cases, bit for bit.  Elements whose scaled magnitudes are in [2^-6, 240) take
+// the hardware's E4M3 conversion, which rounds that range to nearest even like the cache format does.
+// Smaller ones (one lane in thirty for normal values of deviation 12 to 24) have their bytes replaced
+// by the format's: a multiple of 2^-9, rounded half up, masked to three bits, zero below 2^-9.  Eight
+// elements with any larger one, an infinity or a NaN go to the format's own encoder, and only they can
+// hold an exponent field of 15 (`odd`).
+// x / scale is rounded to fp32 as IEEE division does, by Markstein's correction (IBM J. Res. Dev. 34,
+// 1990): with y the correctly rounded reciprocal, q = x y and
+// q + (x - q scale) y is the correctly rounded quotient as long as nothing under- or overflows.
+// `scale` in [2^-60, 2^60] and a quotient of at least 2^-10 make sure of that; below it the bytes are
+// zeros with the element's sign either way.  8192 tokens, 64/8 heads: 78 us with eight elements in the
+// format's encoder for one small one, 73.4 so.
 template <bool F16>
-__device__ __forceinline__ uint2 quantise_row8(uint4 v, float scale, float recip) {
+__device__ __forceinline__ uint2 quantise_row8(uint4 v, float scale, float recip, bool &odd) {
+  constexpr uint32_t kSmall = F16 ? 0x2400u : 0x3c80u, kLarge = F16 ? 0x5b80u : 0x4370u;  // 2^-6, 240
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float t[8];
-  bool usual = recip != 0.f;
+  uint32_t r[4], least = 0xffffffffu, most = 0u;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const float x0 = elem_value<F16>(w[i >> 1] & 0xffffu), x1 = elem_value<F16>(w[i >> 1] >> 16);
+  for (int i = 0; i < 4; i++) {
+    const float x0 = elem_value<F16>(w[i] & 0xffffu), x1 = elem_value<F16>(w[i] >> 16);
     float q0 = x0 * recip, q1 = x1 * recip;
     q0 = fmaf(fmaf(-q0, scale, x0), recip, q0);
     q1 = fmaf(fmaf(-q1, scale, x1), recip, q1);
-    const uint32_t r = pack2<F16>(q0, q1);  // to the 16-bit type first, as the plain write does
-    t[i] = elem_value<F16>(r & 0xffffu);
-    t[i + 1] = elem_value<F16>(r >> 16);
-    const float a = fminf(fabsf(t[i]), fabsf(t[i + 1])), b = fmaxf(fabsf(t[i]), fabsf(t[i + 1]));
-    usual = usual && a >= 0x1p-6f && b < 240.f && t[i] == t[i] && t[i + 1] == t[i + 1];
+    r[i] = pack2<F16>(q0, q1);  // to the 16-bit type first, as the plain write does
+    least = min_u16x2(least, r[i] & 0x7fff7fffu);
+    most = max_u16x2(most, r[i] & 0x7fff7fffu);
   }
-  if (!usual) return quantise8<F16>(v, scale);
+  odd = recip == 0.f || (most & 0xffffu) >= kLarge || (most >> 16) >= kLarge;
+  if (odd) {
+    const uint2 b = quantise8<F16>(v, scale);
+    odd = has_exponent15(b);
+    return b;
+  }
   uint32_t o[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     uint16_t h;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(t[2 * i + 1]), "f"(t[2 * i]));
+    if (F16) asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(h) : "r"(r[i]));
+    else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(elem_value<F16>(r[i] >> 16)), "f"(elem_value<F16>(r[i] & 0xffffu)));
     o[i] = h;
+  }
+  if ((least & 0xffffu) < kSmall || (least >> 16) < kSmall) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const float t = fabsf(elem_value<F16>(r[i >> 1] >> (i & 1) * 16 & 0xffffu));
+      // (the sign is the element's: the correction turns -0 into 0)
+      const uint32_t byte = (w[i >> 1] >> (i & 1) * 16 + 8 & 0x80u) | (t < 0x1p-9f ? 0u : (uint32_t)(int)fmaf(t, 512.f, 0.5f) & 7u);
+      if (t < 0x1p-6f) o[i >> 1] = i & 1 ? (o[i >> 1] & 0xffu) | byte << 8 : (o[i >> 1] & 0xff00u) | byte;
+    }
   }
   return make_uint2(o[0] | o[1] << 16, o[2] | o[3] << 16);
 }
@@ -98,7 +126,7 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 // BATCH: rows that a group of lanes computes while as many more are on their way: 2, or 1 where a
 // group has no more (less code to fetch on a path whose time is the latency of one pass through it).
 // (64 registers, so that an SM holds four CTAs: two rows ahead measured 50.8 us on a 8192-token prompt
-// and 22.4 on an FP8 chunk of 2049, four without looking ahead 51.3 and 26.3, three CTAs of 80 registers
+// and 22.4 on an FP8 chunk of 2049 (same inputs each time), four without looking ahead 51.3 and 26.3, three CTAs of 80 registers
 // and four rows ahead 49.6 and 28.7.)
 template <int GW, bool F16, bool FP8, int PAIR, int BATCH>
 __global__ void __launch_bounds__(kThreads, BATCH == 1 ? 3 : 4)
@@ -186,17 +214,30 @@ rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int 
       }
       slot_s[tid] = s;
     }
-    for (int vt = tok; vt < n_tok; vt += kGroups) {
-      for (int r = first; r < n_heads && in_row; r += 1 << share_log) {
-        const elem16 *v = p.v + (t0 + vt) * p.v_stride + (h + r) * D + e0;
-        uint8_t *dst = v_s + (r * tokens + vt) * v_row + e0 * kElem;
-        if (FP8) {
-          const uint2 b = quantise_row8<F16>(*reinterpret_cast<const uint4 *>(v), p.v_scale, v_recip);
-          if (has_exponent15(b) && p.slot_mapping[t0 + vt] >= 0) atomicOr(p.special, 1u);
-          *reinterpret_cast<uint2 *>(dst) = b;
-        } else {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(v) : "memory");
+    for (int vt = tok; vt < n_tok && in_row; vt += kGroups) {
+      const elem16 *const v = p.v + (t0 + vt) * p.v_stride + h * D + e0;
+      uint8_t *const dst = v_s + vt * v_row + e0 * kElem;
+      const int dst_head = tokens * v_row;
+      if (FP8) {
+        for (int r0 = first; r0 < n_heads; r0 += 4 << share_log) {  // four rows on their way at once
+          uint4 rows[4];
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            const int r = r0 + (b << share_log);
+            if (r < n_heads) rows[b] = *reinterpret_cast<const uint4 *>(v + r * D);
+          }
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            const int r = r0 + (b << share_log);
+            if (r >= n_heads) break;
+            bool odd;
+            *reinterpret_cast<uint2 *>(dst + r * dst_head) = quantise_row8<F16>(rows[b], p.v_scale, v_recip, odd);
+            if (odd && p.slot_mapping[t0 + vt] >= 0) atomicOr(p.special, 1u);
+          }
         }
+      } else {
+        for (int r = first; r < n_heads; r += 1 << share_log)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + r * dst_head)), "l"(v + r * D) : "memory");
       }
     }
   }
@@ -298,9 +339,9 @@ rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int 
           if (in_row && write) {
             uint8_t *st = k_s + ((r * tokens + tok) * D + e0) * kElem;
             if (FP8) {
-              const uint2 q8 = quantise_row8<F16>(out, p.k_scale, k_recip);
-              if (has_exponent15(q8) && p.slot_mapping[t] >= 0) atomicOr(p.special, 1u);
-              *reinterpret_cast<uint2 *>(st) = q8;
+              bool odd;
+              *reinterpret_cast<uint2 *>(st) = quantise_row8<F16>(out, p.k_scale, k_recip, odd);
+              if (odd && p.slot_mapping[t] >= 0) atomicOr(p.special, 1u);
             } else {
               *reinterpret_cast<uint4 *>(st) = out;
             }
@@ -384,28 +425,25 @@ struct Shape {
   dim3 grid;
   size_t smem;
 };
-Shape shape_of(const RotateParams &p, int tok_log, bool fp8, int num_sms) {
+Shape shape_of(const RotateParams &p, int tok_log, bool fp8) {
   const int tokens = 1 << tok_log, gw = p.D <= 32 ? 4 : p.D <= 64 ? 8 : p.D <= 128 ? 16 : 32;
   const int share = std::max((kThreads / gw) >> tok_log, 1);  // groups of a token
   const int head_bytes = tokens * (p.D * (fp8 ? 2 : 4) + 16);
   Shape s;
-  // 16 query or 4 kv heads; half of that where the grid would be less than three waves of four CTAs
-  // per SM, whose last is then a larger part of the whole (FP8 chunk of 2049 tokens: 26.3 -> 22.7 us;
-  // the 8192-token prompt, 3.5 waves, 51.3 -> 57.5)
-  for (int part = 1; part <= 2; part++) {
-    s.q_heads = std::min(p.Hq, std::max(16 / part, share));
-    s.kv_heads = std::max(1, std::min({p.Hkv, std::max(4 / part, share), 40960 / head_bytes}));
-    s.kv_ctas = (p.Hkv + s.kv_heads - 1) / s.kv_heads;
-    s.grid = dim3((unsigned)((p.num_tokens + tokens - 1) >> tok_log), (unsigned)(s.kv_ctas + (p.Hq + s.q_heads - 1) / s.q_heads));
-    if ((int64_t)s.grid.x * s.grid.y >= 12 * num_sms) break;
-  }
+  // 16 query and 4 kv heads (half of both: FP8 chunk of 2049 tokens, 64/8 heads, 22.7 -> 24.6 us; two kv
+  // heads: 8192-token prompt, 32/8 heads, 50.6 -> 55; 32 query heads: FP8, 32768 tokens, 64/8 heads, 279 -> 270,
+  // but the prompt 50.6 -> 55)
+  s.q_heads = std::min(p.Hq, std::max(16, share));
+  s.kv_heads = std::max(1, std::min({p.Hkv, std::max(4, share), 40960 / head_bytes}));
+  s.kv_ctas = (p.Hkv + s.kv_heads - 1) / s.kv_heads;
+  s.grid = dim3((unsigned)((p.num_tokens + tokens - 1) >> tok_log), (unsigned)(s.kv_ctas + (p.Hq + s.q_heads - 1) / s.q_heads));
   s.smem = (size_t)s.kv_heads * head_bytes;
   return s;
 }
 
 template <int GW, bool FP8, bool F16, int PAIR>
-cudaError_t launch_pair(const RotateParams &p, int tok_log, int num_sms, cudaStream_t st) {
-  const Shape s = shape_of(p, tok_log, FP8, num_sms);
+cudaError_t launch_pair(const RotateParams &p, int tok_log, cudaStream_t st) {
+  const Shape s = shape_of(p, tok_log, FP8);
   const int share = (kThreads / GW) >> tok_log;
   auto go = [&](auto kernel) { kernel<<<s.grid, kThreads, s.smem, st>>>(p, tok_log, s.q_heads, s.kv_heads, s.kv_ctas); };
   if (share >= s.q_heads && share >= s.kv_heads) go(rope_norm_cache_kernel<GW, F16, FP8, PAIR, 1>);
@@ -413,10 +451,10 @@ cudaError_t launch_pair(const RotateParams &p, int tok_log, int num_sms, cudaStr
   return cudaGetLastError();
 }
 template <int GW, bool FP8, bool F16>
-cudaError_t launch_group(const RotateParams &p, int tok_log, int num_sms, cudaStream_t st) {
-  if (p.rope.interleaved) return launch_pair<GW, FP8, F16, PAIR_LANE>(p, tok_log, num_sms, st);
-  if (p.rope.dims % 16 == 0) return launch_pair<GW, FP8, F16, PAIR_SHUFFLE>(p, tok_log, num_sms, st);
-  return launch_pair<GW, FP8, F16, PAIR_MEMORY>(p, tok_log, num_sms, st);
+cudaError_t launch_group(const RotateParams &p, int tok_log, cudaStream_t st) {
+  if (p.rope.interleaved) return launch_pair<GW, FP8, F16, PAIR_LANE>(p, tok_log, st);
+  if (p.rope.dims % 16 == 0) return launch_pair<GW, FP8, F16, PAIR_SHUFFLE>(p, tok_log, st);
+  return launch_pair<GW, FP8, F16, PAIR_MEMORY>(p, tok_log, st);
 }
 
 }  // namespace
@@ -426,16 +464,16 @@ cudaError_t launch_rope_norm_cache(const RotateParams &p, bool f16, bool fp8, in
   // two CTAs per SM before a CTA takes more than one token
   int tok_log = 4;
   for (; tok_log > 0; tok_log--) {
-    const Shape s = shape_of(p, tok_log, fp8, num_sms);
+    const Shape s = shape_of(p, tok_log, fp8);
     if ((int64_t)s.grid.x * s.grid.y >= 2 * num_sms) break;
   }
   auto go = [&](auto f16_tag) {
     constexpr bool F16 = decltype(f16_tag)::value;
-    if (fp8) return launch_group<16, true, F16>(p, tok_log, num_sms, st);
-    if (p.D <= 32) return launch_group<4, false, F16>(p, tok_log, num_sms, st);
-    if (p.D <= 64) return launch_group<8, false, F16>(p, tok_log, num_sms, st);
-    if (p.D <= 128) return launch_group<16, false, F16>(p, tok_log, num_sms, st);
-    return launch_group<32, false, F16>(p, tok_log, num_sms, st);
+    if (fp8) return launch_group<16, true, F16>(p, tok_log, st);
+    if (p.D <= 32) return launch_group<4, false, F16>(p, tok_log, st);
+    if (p.D <= 64) return launch_group<8, false, F16>(p, tok_log, st);
+    if (p.D <= 128) return launch_group<16, false, F16>(p, tok_log, st);
+    return launch_group<32, false, F16>(p, tok_log, st);
   };
   const cudaError_t e = f16 ? go(std::true_type{}) : go(std::false_type{});
   __atomic_fetch_add(&g_launch_count, 1ull, __ATOMIC_RELAXED);
