@@ -24,7 +24,7 @@
 // multiple of 8 elements: a shuffle) or, for the odd sizes, are read again from global memory.  The
 // value chunk is a transpose of the rows: where a CTA's 16 tokens fill an aligned run of slots it is
 // stored in runs of tokens out of ldmatrix.trans (FP8: byte permutes), otherwise element by element.
-// Measured on one B200: 8192 tokens, 32/8 heads of 128, keys kept, 218 MB in 50.9 us (4.3 TB/s); 2049
+// Measured on one B200: 8192 tokens, 32/8 heads of 128, keys kept, 218 MB in 49.5 us (4.4 TB/s); 2049
 // tokens, 64/8 heads, FP8 write, 84 MB in 22.7 us; one token 4.3 us in a graph.
 #include <algorithm>
 #include <type_traits>
@@ -50,6 +50,24 @@ __device__ __forceinline__ void unpack8(uint4 v, float (&x)[8]) {
 }
 __device__ __forceinline__ bool has_exponent15(uint2 b) {
   return ((((b.x & 0x78787878u) + 0x08080808u) | ((b.y & 0x78787878u) + 0x08080808u)) & 0x80808080u) != 0u;
+}
+// Two fp32 values at a time: 2049 tokens, 32/8 heads, 18.0 -> 16.5 us, 8192 tokens 50.7 -> 49.5 (rows that
+// rotate interleaved pairs and the FP8 division keep single ones: 22.7 us on an FP8 chunk, 24.5 in twos).
+__device__ __forceinline__ uint64_t pair64(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ void unpair64(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 __device__ __forceinline__ uint32_t min_u16x2(uint32_t a, uint32_t b) {
   uint32_t d;
@@ -250,9 +268,12 @@ rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int 
     unpack8<F16>(r, x);
     float inv = 1.f;
     if (weight) {
-      float ss = 0.f;
+      uint64_t ss2 = 0;
 #pragma unroll
-      for (int i = 0; i < 8; i++) ss = fmaf(x[i], x[i], ss);
+      for (int i = 0; i < 8; i += 2) ss2 = fma2(pair64(x[i], x[i + 1]), pair64(x[i], x[i + 1]), ss2);
+      float ss, ss_odd;
+      unpair64(ss2, ss, ss_odd);
+      ss += ss_odd;
 #pragma unroll
       for (int o = GW / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
       inv = rsqrtf(fmaf(ss, inv_d, p.eps));
@@ -275,9 +296,18 @@ rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int 
       __syncwarp(lanes);  // the row may be rotated in place: all of it has been read
     }
     uint32_t out[4];
+    const uint64_t inv2 = pair64(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2)
-      out[i >> 1] = pack2<F16>(fmaf(x[i], A[i], z[i] * B[i]) * inv, fmaf(x[i + 1], A[i + 1], z[i + 1] * B[i + 1]) * inv);
+    for (int i = 0; i < 8; i += 2) {
+      if (PAIR == PAIR_LANE) {  // (a swapped pair would have to be moved into place)
+        out[i >> 1] = pack2<F16>(fmaf(x[i], A[i], z[i] * B[i]) * inv, fmaf(x[i + 1], A[i + 1], z[i + 1] * B[i + 1]) * inv);
+        continue;
+      }
+      const uint64_t zb = mul2(pair64(z[i], z[i + 1]), pair64(B[i], B[i + 1]));
+      float y0, y1;
+      unpair64(mul2(fma2(pair64(x[i], x[i + 1]), pair64(A[i], A[i + 1]), zb), inv2), y0, y1);
+      out[i >> 1] = pack2<F16>(y0, y1);
+    }
     return make_uint4(out[0], out[1], out[2], out[3]);
   };
   for (;;) {
