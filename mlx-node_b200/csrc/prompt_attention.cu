@@ -44,7 +44,8 @@
 // A probability of a masked key is exactly 0, but 0 * NaN is NaN: a row whose result is not
 // finite is checked for masked values that are not, and then recomputed by itself over the keys
 // that it sees (repair_row).  So is a bf16 row that is not finite after a sum above 2^60 (a logit
-// 41 above everything in the tiles before).  The check costs a comparison per output element.
+// 41 above everything in the tiles before); a sum that overflows makes its row NaN (reciprocal).  The check
+// costs a comparison per output element.
 //
 // Bound by the chain of one query tile (S - softmax - P.V - S), 3200 cycles per 128 keys of both
 // query tiles against 2350 of tensor pipe; measured on one B200: 8192-token prompt, 32/8 heads of
@@ -320,6 +321,12 @@ __device__ __forceinline__ void redo_meet(uint32_t mine, uint32_t other, uint32_
 // 32-column chunks of O: the first half of them is one thread's of a row, the rest the other's.
 __device__ __forceinline__ int chunk_begin(int D, int half) { return half ? (((D + 31) >> 5) + 1) >> 1 : 0; }
 __device__ __forceinline__ int chunk_end(int D, int half) { return half ? (D + 31) >> 5 : (((D + 31) >> 5) + 1) >> 1; }
+
+// 1 / x of a sum of probabilities, NaN for one that has left fp32: bf16 sums may, with every probability and
+// weighted sum inside it still, and 1 / inf = 0 would turn the row into zeros that look like a result.  NaN
+// sticks to the row's sum and reaches every column of it, whatever later tiles, places and pieces add, and the row is
+// recomputed at the end.
+__device__ __forceinline__ float reciprocal(float x) { return 1.f / x + (x - x); }
 
 // O of this half's columns, times a factor per row.
 __device__ __forceinline__ void scale_o(uint32_t o_t, int D, int half, float factor) {
@@ -758,7 +765,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
           if (__any_sync(0xffffffffu, valid && both > 256.f)) {
             float factor = 1.f;
             if (valid && both > 256.f) {
-              factor = 1.f / both;
+              factor = reciprocal(both);
               ref += log2f(both);
             }
             // O holds the tiles before this one: S of this tile was issued after their P.V
@@ -898,7 +905,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         tc_fence_before();
         quad_sync();
       }
-      const float inv = whole ? (l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l)) : 1.f;
+      const float inv = whole ? (l == 0.f ? 0.f : reciprocal(l)) : 1.f;
       constexpr int kRows = 128 * Z::QT;
       float *part = L.ws + (size_t)(2 * blockIdx.x + (g.kt0 > 0 ? 0 : 1)) * (D + 3) * kRows + i * 128 + row;
       bool finite = true;
@@ -1057,7 +1064,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
   for (int c = 0; c < pieces; c++) mx = fmaxf(mx, m_s[c][lane]);
   const float base = mx == -INFINITY ? 0.f : mx;
   for (int c = 0; c < pieces; c++) l += fast_exp2(m_s[c][lane] - base) * l_s[c][lane];
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const float inv = l == 0.f ? 0.f : reciprocal(l);
   elem16 *orow = p.out + (int64_t)(p.cu_q[it.seq] + token) * p.out_stride + (int64_t)(it.head * G + head_in) * D;
   for (int d = warp * 8; d < D; d += 64) {
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

@@ -1,0 +1,72 @@
+"""GPU tests of pa_prompt_attention where logits jump by about as much as fp32's exponent holds.
+
+A tile's probabilities are taken against a reference that the tiles before it set.  In bf16 they
+and their sum may then reach fp32's largest numbers: 88.7 nats above the reference is 2^128.
+Heights here are in nats above the other logits; the tolerance is attend_bound of
+test_gpu_prompt_path, whose 2^-13 covers what logits of this size add: a dot product's rounding and
+that of logit - reference (2^-17 for numbers around 128), a logarithm's and its exponential's
+(the same again), and a reciprocal below 2^-126, which keeps 22 bits.
+"""
+import pytest
+import torch
+
+from test_gpu_prompt_path import Attend
+
+pytestmark = pytest.mark.gpu
+
+# (query lengths, key lengths): one query tile on two places, two query tiles, both of three key tiles
+# and never cut; then items that are cut, and many of which some are
+SHAPES = {
+    "places": ([20], [384]),
+    "tiles": ([64], [384]),
+    "cut": ([20], [1024]),
+    "cut-tiles": ([64], [1024]),
+    "many": ([20] * 90, [512] * 90),
+    "prompt": ([700, 33], [1024, 1024]),
+}
+
+
+def raised(shape, head, heights, f16=False, v_scale=0.1, seed=0):
+    """Attend over `shape` with key j of every sequence `heights(j, kv_len, seq)` nats above the rest."""
+    q, kv = SHAPES[shape]
+    r = Attend(q, kv, 8, 2, head, f16=f16, seed=seed, qk=0.2)
+    r.v = (r.v.float() * v_scale).to(r.v.dtype)
+    r.q[..., :2] = 8.0
+    r.k[..., :2] = 0.0
+    unit = head ** 0.5 / 8
+    for s, base in enumerate(r.cu_kv[:-1]):
+        for j, height in heights(kv[s], s):
+            x = torch.tensor(height * unit)
+            hi = x.to(r.k.dtype)  # in two elements, so that a height is met to a few thousandths
+            r.k[int(base) + j, :, 0] = hi
+            r.k[int(base) + j, :, 1] = (x - hi.float()).to(r.k.dtype)
+    return r
+
+
+def spread(tile, n):
+    """n keys over both halves of a key tile."""
+    return [tile * 128 + i * 128 // n for i in range(n)]
+
+
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("head", [64, 128, 192])
+@pytest.mark.parametrize("n", [2, 16, 128])
+def test_sums_around_the_largest_number(cuda_device, shape, head, n):
+    """Several equal keys whose probabilities, or only their sum, leave fp32 - in the last key tile, in the one
+    before it, and in the second one."""
+    for height in (83.0, 84.6, 85.3, 86.0, 87.2, 88.0, 88.4, 88.6, 89.0):
+        for tile in (-1, -2, 1):
+            r = raised(shape, head, lambda kv, s: [(j, height) for j in spread(tile % (kv // 128), n)])
+            r.run()
+            r.check()
+
+
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("head", [64, 128, 192])
+def test_one_half_of_the_columns_overflows(cuda_device, shape, head):
+    """Values that take one half of a row's outputs beyond fp32 in the last key tile and leave the other there."""
+    for height in (70.0, 84.6, 88.4):
+        r = raised(shape, head, lambda kv, s: [(j, height) for j in spread(kv // 128 - 1, 16)])
+        r.v[..., :head // 2] = (r.v[..., :head // 2].float() * 2.0 ** 40).to(r.v.dtype)
+        r.run()
+        r.check()
