@@ -859,7 +859,23 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         l = half == 0 ? l + l_other : l_other + l;
         if (!F16) far |= get(4) != 0.f;
       }
-      if (both_places && g.kt0 + 1 < g.kt1) {
+      const bool two = both_places && g.kt0 + 1 < g.kt1;
+      if constexpr (!F16) {
+        // What is joined with other parts of its item - the other place, or pieces of other CTAs - is
+        // weighted by 2^(reference - largest reference), and a reference that a jump in the last key tile left
+        // behind by more than fp32's exponents would take its part, of a sum as large, with it.
+        if ((two || g.kt1 - g.kt0 < g.n) && __any_sync(0xffffffffu, valid && far)) {
+          float factor = 1.f;
+          if (valid && far) {
+            factor = reciprocal(l);
+            ref += log2f(l);
+            l *= factor;
+          }
+          scale_o(o_t, D, half, factor);
+          tmem_wait_st();
+        }
+      }
+      if (two) {
         // place 1 hands its reference and sum to place 0, which reads both accumulators
         auto quad_sync = [&] { asm volatile("bar.sync %0, 128;" ::"r"(9 + quad) : "memory"); };
         if (i == 1) {

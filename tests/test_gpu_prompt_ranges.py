@@ -70,3 +70,30 @@ def test_one_half_of_the_columns_overflows(cuda_device, shape, head):
         r.v[..., :head // 2] = (r.v[..., :head // 2].float() * 2.0 ** 40).to(r.v.dtype)
         r.run()
         r.check()
+
+
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("head", [64, 128, 192])
+@pytest.mark.parametrize("f16", [False, True])
+def test_parts_with_references_far_apart(cuda_device, shape, head, f16):
+    """Key tiles of any height: the pieces and places of an item end with references up to fp32's exponent range
+    and more apart, while the sums of those left behind make up for it."""
+    heights = (0.0, 60.0, 80.0, 86.0, 87.0, 87.5, 88.0, 89.0, 91.0, 120.0, 176.0)
+    for seed in range(12):
+        pick = torch.randint(0, len(heights), (128, 64), generator=torch.Generator().manual_seed(seed)).tolist()
+
+        def tiles(kv, s):
+            return [(j, heights[pick[s][t]]) for t in range(1, kv // 128) for j in spread(t, 1 + pick[s][63 - t] % 3)]
+        r = raised(shape, head, tiles, f16=f16, seed=seed)
+        r.run()
+        r.check()
+
+
+@pytest.mark.parametrize("head", [64, 128])
+def test_two_places_far_apart(cuda_device, head):
+    """Tiles 0 and 2 share a place, tile 1 has its own: the sum of the first, 2^125 against a reference of 0,
+    next to a reference of 2^127."""
+    for low, high in ((87.0, 88.0), (88.4, 90.0), (86.0, 89.0)):
+        r = raised("places", head, lambda kv, s: [(200, high), (260, low)])
+        r.run()
+        r.check()
