@@ -43,8 +43,8 @@
 //
 // A probability of a masked key is exactly 0, but 0 * NaN is NaN: a row whose result is not
 // finite is checked for masked values that are not, and then recomputed by itself over the keys
-// that it sees (repair_row).  So is a bf16 row that is not finite after a sum above 2^60 (a logit
-// 41 above everything in the tiles before); a sum that overflows makes its row NaN (reciprocal).  The check
+// that it sees (repair_row).  So is a bf16 row that is not finite after a sum above 2^16 (a logit
+// 11 above everything in the tiles before); a sum that overflows makes its row NaN (reciprocal).  The check
 // costs a comparison per output element.
 //
 // Bound by the chain of one query tile (S - softmax - P.V - S), 3200 cycles per 128 keys of both
@@ -661,8 +661,9 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
     const float cap_in = p.scale / p.softcap, cap_out = p.softcap / p.scale;
     // Sums of up to this much against the stale reference are taken as they are.  f16 ends at 2^16; bf16 has
     // fp32's range, and its probabilities are announced before the sum is known.
-    // (bf16: beyond this a row that comes out not finite is recomputed, see `far`)
-    constexpr float kFar = F16 ? 32768.f : 1.152921504606847e18f;
+    // (bf16: beyond this a row that comes out not finite is recomputed, see `far`.  Its weighted sums are as
+    // far above the result as the sum is above 1: below this, values of up to 2^110 stay in fp32.)
+    constexpr float kFar = F16 ? 32768.f : 65536.f;
     auto put = [&](uint32_t slot, float x) { asm volatile("st.volatile.shared.f32 [%0], %1;" ::"r"(mine + slot * kSlot), "f"(x) : "memory"); };
     auto get = [&](uint32_t slot) {
       float y;
@@ -709,7 +710,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
       float ref = 0.f, l = 0.f, sum = 0.f;  // ref: 0 while the row has seen nothing
       bool behind = false;  // tile cnt - 1 is this item's, and the other warp may yet call a meeting about it
       int left = 0;         // columns of the tile from here on are masked
-      bool far = false;     // bf16: a sum was so large that an overflow is this kernel's own
+      bool far = false;     // bf16: a sum was so large that an overflow may be this kernel's own
       [[maybe_unused]] auto redo = [&](bool stored, bool rescale) {
         const uint32_t tile = stored ? cnt - 1 : cnt;
         const Redo r = redo_tile<CAP, F16>(s_t, o_t, D, half, c, cap_in, cap_out, ref, l, sum, mine + (tile & 1) * kSlot,

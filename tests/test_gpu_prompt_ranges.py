@@ -97,3 +97,16 @@ def test_two_places_far_apart(cuda_device, head):
         r = raised("places", head, lambda kv, s: [(200, high), (260, low)])
         r.run()
         r.check()
+
+
+@pytest.mark.parametrize("shape", list(SHAPES))
+@pytest.mark.parametrize("log2_v", [40, 90, 100])
+def test_large_values_behind_a_jump(cuda_device, shape, log2_v):
+    """bf16 values of up to 2^100: probabilities far above 1 would take the weighted sum beyond fp32 although the
+    result is inside."""
+    for height in (15.0, 30.0, 45.0):
+        for tile in (-1, 1):
+            r = raised(shape, 128, lambda kv, s: [(j, height) for j in spread(tile % (kv // 128), 2)],
+                       v_scale=2.0 ** log2_v)
+            r.run()
+            r.check()
