@@ -199,9 +199,13 @@ def _ptr(x) -> int:
         return data_ptr()
     if isinstance(x, int):
         return x
-    array = getattr(x, "__array_interface__", None)  # numpy array (host memory)
-    if array is not None:
-        return array["data"][0]
+    # numpy array (host memory).  Its class says so: numpy's scalars have an __array_interface__ too, of
+    # a copy that is freed before the call could use it
+    if hasattr(type(x), "ctypes"):
+        array = getattr(x, "__array_interface__", None)
+        return x.ctypes.data if array is None else array["data"][0]
+    if hasattr(x, "ctypes"):
+        return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
