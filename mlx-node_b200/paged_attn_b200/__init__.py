@@ -190,8 +190,8 @@ def _check(status: int) -> None:
 
 
 def _ptr(x) -> int:
-    # in the order of how often a call passes them: a call's own time on the host is a few
-    # microseconds, of which a numpy array's .ctypes alone would be one
+    # in the order of how often a call passes them, each attribute looked up once: a call's own time on
+    # the host is a few microseconds, of which a numpy array's .ctypes is one
     if x is None:
         return 0
     data_ptr = getattr(x, "data_ptr", None)
@@ -199,13 +199,11 @@ def _ptr(x) -> int:
         return data_ptr()
     if isinstance(x, int):
         return x
-    # numpy array (host memory).  Its class says so: numpy's scalars have an __array_interface__ too, of
-    # a copy that is freed before the call could use it
-    if hasattr(type(x), "ctypes"):
-        array = getattr(x, "__array_interface__", None)
-        return x.ctypes.data if array is None else array["data"][0]
-    if hasattr(x, "ctypes"):
-        return x.ctypes.data
+    # numpy array (host memory); numpy's scalars have no .ctypes, only an __array_interface__ of a copy
+    # that is freed before the call could use it
+    address = getattr(x, "ctypes", None)
+    if address is not None:
+        return address.data
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
