@@ -226,9 +226,11 @@ __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 6
 
 // One row - a (query token, query head) - by one warp over exactly the keys it sees: 32 keys
 // at a time, a lane per key for the logits, the online softmax across the warp, then a lane per
-// output dimension.  Writes the 8-column pieces whose bit is set in `pieces`.
+// output dimension.  Writes the 8-column pieces whose bit is set in `pieces`; counts every 16384 keys in
+// `beat` (null: nobody waits), as millions of keys take longer than a wait's second.
 template <bool F16>
-__device__ __noinline__ void repair_row(const PromptParams &p, int s, int token, int head, uint32_t pieces) {
+__device__ __noinline__ void repair_row(const PromptParams &p, int s, int token, int head, uint32_t pieces,
+                                        volatile uint32_t *beat) {
   const int lane = threadIdx.x & 31, D = p.D, h = head / p.G;
   const int q_len = p.cu_q[s + 1] - p.cu_q[s], kv_len = p.cu_kv[s + 1] - p.cu_kv[s];
   const int keys = kv_len - q_len + token + 1;
@@ -236,6 +238,7 @@ __device__ __noinline__ void repair_row(const PromptParams &p, int s, int token,
   elem16 *out = p.out + (int64_t)(p.cu_q[s] + token) * p.out_stride + (int64_t)head * D;
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
   for (int j0 = 0; j0 < keys; j0 += 32) {
+    if (beat && (j0 & 16383) == 0 && lane == 0) atomicAdd(const_cast<uint32_t *>(beat), 1u);
     const int j = j0 + lane;
     float x = -INFINITY;
     if (j < keys) {
@@ -1009,7 +1012,7 @@ prompt_attention_kernel(const __grid_constant__ PromptLaunch L, const __grid_con
         if (own || masked_value_not_finite(p, g.s, tk, g.h, g.n, F16)) {
           // pieces of eight columns, four to a chunk
           const uint32_t below = (uint32_t)((1ull << (c0 * 4)) - 1), upto = (uint32_t)((1ull << (c1 * 4)) - 1);
-          repair_row<F16>(p, g.s, tk, hd, upto & ~below);
+          repair_row<F16>(p, g.s, tk, hd, upto & ~below, beat);
         }
         if (lane == 0) atomicAdd(const_cast<uint32_t *>(beat), 1u);
       }
@@ -1117,7 +1120,7 @@ __global__ void __launch_bounds__(256) prompt_join_kernel(const __grid_constant_
       const int src = __ffs(odd) - 1;
       odd &= odd - 1;
       const int tk = __shfl_sync(0xffffffffu, token, src), hd = it.head * G + __shfl_sync(0xffffffffu, head_in, src);
-      if (far_s[src] || masked_value_not_finite(p, it.seq, tk, it.head, n, F16)) repair_row<F16>(p, it.seq, tk, hd, 1u << (d >> 3));
+      if (far_s[src] || masked_value_not_finite(p, it.seq, tk, it.head, n, F16)) repair_row<F16>(p, it.seq, tk, hd, 1u << (d >> 3), nullptr);
     }
   }
 }

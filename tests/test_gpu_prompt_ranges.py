@@ -10,7 +10,7 @@ that of logit - reference (2^-17 for numbers around 128), a logarithm's and its 
 import pytest
 import torch
 
-from test_gpu_prompt_path import Attend
+from test_gpu_prompt_path import Attend, attend_bound, gen
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +110,26 @@ def test_large_values_behind_a_jump(cuda_device, shape, log2_v):
                        v_scale=2.0 ** log2_v)
             r.run()
             r.check()
+
+
+def test_a_recomputed_row_outlasts_a_wait(cuda_device):
+    """One row over two million keys jumps beyond fp32's exponent: recomputing it takes longer than the second that
+    the CTA's other warps wait for anything, which is no error while it gets on.  160 query tiles, so that the
+    row's item is not cut."""
+    n, head, queries = 1 << 21, 256, 160 * 128
+    r = Attend([queries], [128], 1, 1, head)
+    g = gen(1)
+    r.cu_kv[1] = n
+    r.k, r.v = (torch.empty(n, 1, head, dtype=r.q.dtype, device="cuda").normal_(0, s, generator=g) for s in (0.7, 1.0))
+    r.q[..., 0], r.k[..., 0] = 0.0, 0.0
+    r.q[0, 0, 0], r.k[n // 2, 0, 0] = 8.0, 100.0 * head ** 0.5 / 8
+    r.run()
+    torch.cuda.synchronize()
+    r.cache.check_errors()
+    seen = n - queries + 1
+    parts = [slice(i, min(i + (1 << 18), seen)) for i in range(0, seen, 1 << 18)]
+    p = torch.softmax(torch.cat([r.k[s, 0].double() @ r.q[0, 0].double() for s in parts]) * r.scale, 0)
+    ref = sum(p[s] @ r.v[s, 0].double() for s in parts)
+    mag = sum(p[s] @ r.v[s, 0].double().abs() for s in parts)
+    assert ((r.out[0, 0].double() - ref).abs() <= attend_bound(r.q.dtype, ref, mag, n)).all()
+    assert torch.isfinite(r.out[:queries]).all()
