@@ -556,7 +556,8 @@ pa_status pa_paged_attention_varlen(PagedAttnCache *cache, uint32_t layer_idx,
  * cache's q/out type), its pools are not touched.
  *   out, q        [cu_q_lens[num_seqs], num_q_heads, head_size], packed by sequence
  *   k, v          [cu_kv_lens[num_seqs], num_kv_heads, head_size]; row strides of all four
- *                 in elements
+ *                 in elements; out shares no element with q, k and v
+ *                 (one of their pointers given as out is refused)
  *   cu_q_lens_host, cu_kv_lens_host  int32 [num_seqs + 1] in HOST memory, non-decreasing,
  *                 read during the call only (a captured graph replays these lengths);
  *                 cu_kv_lens_host may be null: the same as cu_q_lens_host

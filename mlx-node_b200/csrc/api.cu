@@ -698,6 +698,7 @@ pa_status pa_prompt_attention(PagedAttnCache *c, void *out, const void *q, const
                                              num_q_heads, q_stride, k_stride, v_stride, out_stride, scale,
                                              softcap, workspace, workspace_bytes, pa_prompt_workspace_bytes(c)))
     return arg_fail(e);
+  if (pa::ArgError e = pa::check_prompt_in_place(out, q, k, v)) return arg_fail(e);
   const int32_t *cu_kv = cu_kv_lens_host ? cu_kv_lens_host : cu_q_lens_host;
   pa::PromptParams p{};
   p.out = static_cast<pa::elem16 *>(out);

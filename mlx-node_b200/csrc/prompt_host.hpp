@@ -176,6 +176,13 @@ inline ArgError check_prompt_args(const PagedAttnConfig &cfg, const void *out, c
   return {};
 }
 
+// The output in an input's place: a row that is recomputed reads its query after other lanes have written
+// there, and every row its keys and values after the rows of other CTAs.
+inline ArgError check_prompt_in_place(const void *out, const void *q, const void *k, const void *v) {
+  if (out && (out == q || out == k || out == v)) return bad_arg("out may not be one of the inputs");
+  return {};
+}
+
 inline ArgError check_gather_args(const PagedAttnConfig &cfg, const void *key, const void *value,
                                   const int32_t *block_tables, const int32_t *starts, const int32_t *cu,
                                   int32_t num_seqs, int32_t max_blocks, int64_t key_stride, int64_t value_stride) {
