@@ -287,6 +287,7 @@ pa_status pa_rope_frequencies(const PaRope *rope, double *frequencies, float *ga
  *   q_out        receives the queries; may be q itself with q's stride
  *   k_out        null, or receives the keys [num_tokens, num_kv_heads, head_size]; may be k
  *                itself with k's stride.  No other overlap of inputs and outputs is allowed
+ *                (in place with another stride, or in another tensor's place: refused)
  *   q_norm_weight, k_norm_weight  [head_size] in the cache dtype, or null for no norm
  *   positions    int32 [num_tokens], device; any value
  *   slot_mapping int64 [num_tokens], device, or null: nothing is written to the pool (v may

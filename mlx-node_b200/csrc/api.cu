@@ -603,6 +603,9 @@ pa_status pa_rope_norm_and_cache(PagedAttnCache *c, uint32_t layer, const PaRope
                                              num_tokens, num_q_heads, q_stride, q_out_stride, k_stride,
                                              k_out_stride, v_stride))
     return arg_fail(e);
+  if (pa::ArgError e = pa::check_rotate_in_place(q_out, k_out, q, k, slot_mapping ? v : nullptr, num_tokens, q_stride,
+                                                 q_out_stride, k_stride, k_out_stride))
+    return arg_fail(e);
   pa::RotateParams p{};
   p.q = static_cast<const pa::elem16 *>(q);
   p.k = static_cast<const pa::elem16 *>(k);

@@ -137,6 +137,19 @@ inline ArgError check_rotate_args(const PagedAttnConfig &cfg, const RopeTable *r
   return {};
 }
 
+// Rows rotated in place have to come back to where they were read: with another stride a row's result
+// lands on rows that other lanes have yet to read.
+inline ArgError check_rotate_in_place(const void *q_out, const void *k_out, const void *q, const void *k,
+                                      const void *v, int64_t num_tokens, int64_t q_stride, int64_t q_out_stride,
+                                      int64_t k_stride, int64_t k_out_stride) {
+  if (num_tokens > 1 && q_out == q && q_out_stride != q_stride) return bad_arg("q rotated in place needs one stride");
+  if (num_tokens > 1 && k_out && k_out == k && k_out_stride != k_stride)
+    return bad_arg("k rotated in place needs one stride");
+  if (q_out == k || q_out == v || q_out == k_out || (k_out && (k_out == q || k_out == v)))
+    return bad_arg("outputs may be no other tensor of the call");
+  return {};
+}
+
 inline ArgError check_cu(const int32_t *cu, int32_t n, const char *what) {
   if (cu[0] < 0) return bad_arg(what);
   for (int32_t i = 0; i < n; i++)
