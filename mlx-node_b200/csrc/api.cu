@@ -719,6 +719,9 @@ pa_status pa_prompt_attention(PagedAttnCache *c, void *out, const void *q, const
   p.scale = scale;
   p.softcap = softcap;
   DeviceGuard g(c->device);
+  // A thread that has made no CUDA call yet has this device by default, but no context, which encoding a
+  // tensor map needs: a driver call, unlike a launch, does not bring it up.
+  PA_CUDA(cudaSetDevice(c->device));
   for (int32_t s0 = 0; s0 < num_seqs; s0 += pa::kMaxPlanSeqs) {
     p.S = std::min(num_seqs - s0, pa::kMaxPlanSeqs);
     std::copy(cu_q_lens_host + s0, cu_q_lens_host + s0 + p.S + 1, p.cu_q);
