@@ -44,8 +44,8 @@ __device__ __forceinline__ uint2 dequant4(uint32_t w, float scale256) {
 
 // DC: head dimensions a warp has in flight (32 or 64); more are taken in turns.  64 registers, 32 warps
 // on an SM in CTAs of four that come and go; stores marked streaming, as nothing here is read again.
-// 8 sequences of 2000-8192 tokens, 8 heads of 128: 298 MB in 55.4 us = 5.4 TB/s (CTAs of eight warps,
-// 128 dimensions, plain stores: 59.7); the FP8 ranges 247 MB in 46.2 us (57.0).
+// 8 sequences of 2000-8192 tokens, 8 heads of 128: 298 MB in 52.0 us = 5.7 TB/s (CTAs of eight warps,
+// 128 dimensions, plain stores: 59.7); the FP8 ranges 247 MB in 46.7 us (57.0).
 template <int DC, bool F16, bool FP8>
 __global__ void __launch_bounds__(kWarps * 32, 8) gather_cache_kernel(const __grid_constant__ GatherParams p) {
   __shared__ __align__(128) uint4 v_s[kWarps][DC * 2];  // 16-byte pieces (dimension, token half)

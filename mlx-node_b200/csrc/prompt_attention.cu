@@ -47,10 +47,19 @@
 // 11 above everything in the tiles before); a sum that overflows makes its row NaN (reciprocal).  The check
 // costs a comparison per output element.
 //
+// That recomputation is one warp's scalar work and slow: 0.78 s for a row of a million keys of 256
+// dimensions, and where every row of a prompt of 4096 (8 heads of 128) jumps by 100 nats, 271 ms instead of
+// 62 us.  It takes jumps of 84 to 88.7 nats - the sum's or a probability's exponent - and more over everything before
+// in the row, or a NaN or infinity in a value that the row's last key tiles hold and the row does not see.  f16 jumps are settled in the
+// loop (redo_tile).
+//
 // Bound by the chain of one query tile (S - softmax - P.V - S), 3200 cycles per 128 keys of both
-// query tiles against 2350 of tensor pipe; measured on one B200: 8192-token prompt, 32/8 heads of
-// 128, bf16, 485-540 us (1.0-1.1 PFLOP/s); two chunks of 1024 over 4096 163-169 us; eight sequences
-// of 1-5 tokens over 4000-16000 keys 72-80 us (4.5-4.9 TB/s).
+// query tiles against 2350 of tensor pipe; measured on several B200s, with the same and
+// with changing inputs: 8192-token prompt, 32/8 heads of 128, bf16, 467-550 us (1.0-1.18 PFLOP/s); seven f16 prompts of 700-2500 260-311 us; two
+// chunks of 1024 over 4096 160-173 us; eight sequences of 1-5 tokens over 4000-16000 keys 75-81 us (4.4-4.8 TB/s).
+// The 8192-token prompt in other forms: f16 530 us, softcap 1230 (a tanhf per logit), head size 64 412 us, 16/4
+// heads of 192 429 and of 256 517 (f16 613).  The two-tile kernels hold 96 registers a thread and spill: 20 bytes
+// of reloads in bf16, 136 in f16, which keeps what redo_tile needs.
 //
 // Every wait is bounded; on expiry the CTA raises the error word, every role leaves its loop,
 // copies in flight are drained and TMEM is freed.

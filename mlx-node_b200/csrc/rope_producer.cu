@@ -24,8 +24,12 @@
 // multiple of 8 elements: a shuffle) or, for the odd sizes, are read again from global memory.  The
 // value chunk is a transpose of the rows: where a CTA's 16 tokens fill an aligned run of slots it is
 // stored in runs of tokens out of ldmatrix.trans (FP8: byte permutes), otherwise element by element.
-// Measured on one B200: 8192 tokens, 32/8 heads of 128, keys kept, 218 MB in 49.5 us (4.4 TB/s); 2049
-// tokens, 64/8 heads, FP8 write, 84 MB in 22.7 us; one token 4.3 us in a graph.
+// Measured on one B200, the same inputs over and over: 8192 tokens, 32/8 heads of 128, keys kept, 218 MB in
+// 50.0 us (4.4 TB/s) where the slots begin with a block; 53.4 where they begin inside one, 52.1 as packed
+// prompts of 300-900 tokens, 51.4 with blocks of 8 tokens (the element-wise write); 47.5 with interleaved pairs; 89.7
+// with 90 of the 128 elements rotated (partners read again).  2049 tokens, 64/8 heads, FP8 write, 84 MB in 20.7 us,
+// 21.3 from inside a block; with changing inputs 50.6 and 22.7.  64 tokens in a graph 6.0 us in a row and 6.1 with a
+// block and a position each; one token 4.3.
 #include <algorithm>
 #include <type_traits>
 
@@ -145,7 +149,8 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 // group has no more (less code to fetch on a path whose time is the latency of one pass through it).
 // (64 registers, so that an SM holds four CTAs: two rows ahead measured 50.8 us on a 8192-token prompt
 // and 22.4 on an FP8 chunk of 2049 (same inputs each time), four without looking ahead 51.3 and 26.3, three CTAs of 80 registers
-// and four rows ahead 49.6 and 28.7.)
+// and four rows ahead 49.6 and 28.7.  At 64 registers the form with two rows ahead spills, in stores per thread: 32 to
+// 64 bytes with 16-bit pools, 56 to 88 with FP8, 124 to 144 where partners are read again.)
 template <int GW, bool F16, bool FP8, int PAIR, int BATCH>
 __global__ void __launch_bounds__(kThreads, BATCH == 1 ? 3 : 4)
 rope_norm_cache_kernel(const __grid_constant__ RotateParams p, int tok_log, int q_heads, int kv_heads, int kv_ctas) {
